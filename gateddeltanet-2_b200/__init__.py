@@ -10,6 +10,15 @@ Drop-in for the reference's ``lit_gpt.gdn2_ops``:
 * ``GatedDeltaNet2`` — the token-mixer layer around the operator
   (``lit_gpt/gdn2.py``), with its fused prep and gated-norm kernels.
 
+Beside them, without a reference counterpart:
+
+* ``chunk_linear_attn`` / ``fused_recurrent_linear_attn`` — linear attention
+  with a decay for each head: chunkwise forward + backward, and the
+  token-serial form for decoding;
+* ``layer_norm`` / ``LayerNorm`` — layer norm with an optional residual add,
+  forward + backward;
+* ``LinearAttention`` — the token mixer that runs them together.
+
 Every op runs hand-written CUDA in ``libgdn2_b200.so`` through the C ABI
 declared in ``include/gdn2.h``; there is no CPU or Triton fallback.
 
@@ -23,6 +32,9 @@ import sys as _sys
 from . import _lib, cp
 from .chunk import ChunkGDN2Function, chunk_gdn2, gdn2_telemetry_snapshot, prepare_chunk_indices
 from .layer import FusedRMSNormSwishGate, GatedDeltaNet2, LayerCache, ShortConvolution
+from .layer_norm import LayerNorm, LayerNormFunction, layer_norm
+from .linear_attn import ChunkLinearAttnFunction, chunk_linear_attn, fused_recurrent_linear_attn
+from .linear_layer import LinearAttention
 from .recurrent import fused_recurrent_gdn2, fused_recurrent_gdn2_fwd
 
 _sys.modules.setdefault("gdn2_b200", _sys.modules[__name__])
@@ -39,4 +51,11 @@ __all__ = [
     "LayerCache",
     "ShortConvolution",
     "FusedRMSNormSwishGate",
+    "chunk_linear_attn",
+    "ChunkLinearAttnFunction",
+    "fused_recurrent_linear_attn",
+    "layer_norm",
+    "LayerNorm",
+    "LayerNormFunction",
+    "LinearAttention",
 ]

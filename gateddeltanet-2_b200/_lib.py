@@ -30,6 +30,8 @@ G_BF16 = 1 << 8
 SKIP_INTRA = 1 << 9
 # enum gdn2_ws_buffer
 WS_CHUNK_STATES = 0
+# enum gdn2_decay
+DECAY_NONE, DECAY_HEAD, DECAY_TOKEN = 0, 1, 2
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -88,6 +90,42 @@ class PrepGrads(ctypes.Structure):
     ]
 
 
+_s3 = _i64 * 3
+
+
+class LinearAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", _i64), ("T", _i64), ("H", _i64), ("HV", _i64), ("K", _i64), ("V", _i64),
+        ("N", _i64),
+        ("q_stride", _s3), ("k_stride", _s3), ("v_stride", _s3), ("g_stride", _s3),
+        ("cu_seqlens", _p), ("state_indices", _p), ("num_slots", _i64),
+        ("state_stride_in", _i64), ("state_stride_out", _i64),
+        ("scale", _f32), ("flags", _i32), ("dtype", _i32), ("dtype_g", _i32), ("decay", _i32),
+        ("q", _p), ("k", _p), ("v", _p), ("g", _p), ("h0", _p), ("ht", _p), ("o", _p),
+    ]
+
+
+class LinearAttnGrads(ctypes.Structure):
+    _fields_ = [
+        ("dout", _p), ("dht", _p), ("dq", _p), ("dk", _p), ("dv", _p), ("dg", _p), ("dh0", _p),
+    ]
+
+
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64), ("D", _i64), ("eps", _f32),
+        ("dtype", _i32), ("dtype_residual", _i32), ("dtype_weight", _i32),
+        ("x", _p), ("residual", _p), ("weight", _p), ("bias", _p), ("y", _p), ("s", _p),
+        ("mean", _p), ("rstd", _p),
+    ]
+
+
+class LayerNormGrads(ctypes.Structure):
+    _fields_ = [
+        ("dy", _p), ("ds", _p), ("s", _p), ("dx", _p), ("dresidual", _p), ("dweight", _p), ("dbias", _p),
+    ]
+
+
 class KernelStat(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("launches", _i64), ("total_ms", ctypes.c_double)]
 
@@ -108,6 +146,9 @@ EXPORTS = (
     "gdn2_profile_enable", "gdn2_profile_read", "gdn2_device_fault_read",
     "gdn2_layer_prep_fwd", "gdn2_layer_prep_bwd_workspace_size", "gdn2_layer_prep_bwd",
     "gdn2_norm_gate_fwd", "gdn2_norm_gate_bwd_workspace_size", "gdn2_norm_gate_bwd",
+    "gdn2_linear_attn_workspace_size", "gdn2_linear_attn_fwd", "gdn2_linear_attn_bwd_workspace_size",
+    "gdn2_linear_attn_bwd", "gdn2_linear_attn_recurrent_fwd",
+    "gdn2_layer_norm_fwd", "gdn2_layer_norm_bwd_workspace_size", "gdn2_layer_norm_bwd",
 )
 
 
@@ -165,6 +206,24 @@ def load() -> ctypes.CDLL:
     lib.gdn2_norm_gate_bwd_workspace_size.restype = ctypes.c_size_t
     lib.gdn2_norm_gate_bwd.argtypes = [_p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, ctypes.c_size_t, _p]
     lib.gdn2_norm_gate_bwd.restype = ctypes.c_int
+    la, lg = ctypes.POINTER(LinearAttnArgs), ctypes.POINTER(LinearAttnGrads)
+    lib.gdn2_linear_attn_workspace_size.argtypes = [la]
+    lib.gdn2_linear_attn_workspace_size.restype = ctypes.c_size_t
+    lib.gdn2_linear_attn_fwd.argtypes = [la, _p, ctypes.c_size_t, _p]
+    lib.gdn2_linear_attn_fwd.restype = ctypes.c_int
+    lib.gdn2_linear_attn_bwd_workspace_size.argtypes = [la]
+    lib.gdn2_linear_attn_bwd_workspace_size.restype = ctypes.c_size_t
+    lib.gdn2_linear_attn_bwd.argtypes = [la, lg, _p, ctypes.c_size_t, _p, ctypes.c_size_t, _p]
+    lib.gdn2_linear_attn_bwd.restype = ctypes.c_int
+    lib.gdn2_linear_attn_recurrent_fwd.argtypes = [la, _p]
+    lib.gdn2_linear_attn_recurrent_fwd.restype = ctypes.c_int
+    na, ng = ctypes.POINTER(LayerNormArgs), ctypes.POINTER(LayerNormGrads)
+    lib.gdn2_layer_norm_fwd.argtypes = [na, _p]
+    lib.gdn2_layer_norm_fwd.restype = ctypes.c_int
+    lib.gdn2_layer_norm_bwd_workspace_size.argtypes = [na]
+    lib.gdn2_layer_norm_bwd_workspace_size.restype = ctypes.c_size_t
+    lib.gdn2_layer_norm_bwd.argtypes = [na, ng, _p, ctypes.c_size_t, _p]
+    lib.gdn2_layer_norm_bwd.restype = ctypes.c_int
     _lib = lib
     return lib
 
@@ -181,6 +240,24 @@ def ptr(t) -> int | None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """``torch.cuda.device`` without its cost where the device is current already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device):
+        here = device.index is None or device.index == torch.cuda.current_device()
+        self.guard = None if here else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 _checked_devices: set[int] = set()
@@ -208,8 +285,8 @@ def profile_enable(on: bool) -> None:
 
 def profile_read() -> dict:
     """{kernel name: (launches, total device ms)} since the last read."""
-    buf = (KernelStat * 16)()
-    n = load().gdn2_profile_read(buf, 16)
+    buf = (KernelStat * 64)()
+    n = load().gdn2_profile_read(buf, 64)
     if n < 0:
         check(n, "gdn2_profile_read")
     return {buf[i].name.decode(): (int(buf[i].launches), float(buf[i].total_ms)) for i in range(n)}

@@ -2,6 +2,7 @@
 // workspace carving and dispatch.  Nothing here allocates device memory.
 #include "chunk_layout.cuh"
 #include "common.cuh"
+#include "linear_attn.cuh"
 
 using namespace gdn2;
 
@@ -42,11 +43,48 @@ int check_chunk(const gdn2_chunk_args* a, bool need_ptrs = true, bool need_out =
   return GDN2_OK;
 }
 
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+// the arguments that the chunkwise and the recurrent linear attention share
+int check_linear_attn(const gdn2_linear_attn_args* a, bool need_ptrs, bool need_out) {
+  if (!a) return GDN2_ERR_NULL_POINTER;
+  if (a->B < 0 || a->T < 0 || a->H <= 0 || a->HV <= 0 || a->N < 0 || a->HV % a->H) return GDN2_ERR_SHAPE;
+  if (a->HV > 65535 || a->B * a->T >= (int64_t(1) << 31) || a->N >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
+  if (!dim_ok(a->K) || !dim_ok(a->V)) return GDN2_ERR_UNSUPPORTED_DIM;
+  if (a->dtype != GDN2_BF16 && a->dtype != GDN2_F32) return GDN2_ERR_DTYPE;
+  if (a->decay < GDN2_DECAY_NONE || a->decay > GDN2_DECAY_TOKEN) return GDN2_ERR_FLAGS;
+  if (a->decay != GDN2_DECAY_NONE && a->dtype_g != GDN2_BF16 && a->dtype_g != GDN2_F32) return GDN2_ERR_DTYPE;
+  if (a->flags & ~(GDN2_HAS_H0 | GDN2_STORE_FINAL | GDN2_SAVE_FOR_BWD)) return GDN2_ERR_FLAGS;
+  if (a->cu_seqlens ? a->B != 1 : a->N != a->B) return GDN2_ERR_SHAPE;
+  if (!need_ptrs) return GDN2_OK;
+  if ((a->flags & GDN2_HAS_H0) && !a->h0) return GDN2_ERR_NULL_POINTER;
+  if (need_out && (a->flags & GDN2_STORE_FINAL) && !a->ht) return GDN2_ERR_NULL_POINTER;
+  if (misaligned(a->h0) || misaligned(a->ht)) return GDN2_ERR_ALIGNMENT;
+  if (a->B * a->T == 0) return GDN2_OK;
+  if (!a->q || !a->k || !a->v || (need_out && !a->o) || (a->decay != GDN2_DECAY_NONE && !a->g))
+    return GDN2_ERR_NULL_POINTER;
+  if (misaligned(a->q) || misaligned(a->k) || misaligned(a->v) || misaligned(a->o)) return GDN2_ERR_ALIGNMENT;
+  const int64_t per = a->dtype == GDN2_BF16 ? 8 : 4;
+  for (int i = 0; i < 3; ++i)
+    if (a->q_stride[i] % per || a->k_stride[i] % per || a->v_stride[i] % per) return GDN2_ERR_ALIGNMENT;
+  return GDN2_OK;
+}
+
+int check_layer_norm(const gdn2_layer_norm_args* a) {
+  if (!a) return GDN2_ERR_NULL_POINTER;
+  if (a->rows < 0 || a->rows >= (int64_t(1) << 31) || a->D < 1) return GDN2_ERR_SHAPE;
+  if (a->D > 32768) return GDN2_ERR_UNSUPPORTED_DIM;
+  if (a->dtype != GDN2_BF16 && a->dtype != GDN2_F32) return GDN2_ERR_DTYPE;
+  if ((a->weight || a->bias) && a->dtype_weight != GDN2_BF16 && a->dtype_weight != GDN2_F32) return GDN2_ERR_DTYPE;
+  if (a->residual && a->dtype_residual != GDN2_F32 && a->dtype_residual != a->dtype) return GDN2_ERR_DTYPE;
+  return GDN2_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
-int gdn2_abi_version(void) { return 100; }
+int gdn2_abi_version(void) { return 101; }
 
 const char* gdn2_status_string(int s) {
   switch (s) {
@@ -54,7 +92,7 @@ const char* gdn2_status_string(int s) {
     case GDN2_ERR_NULL_POINTER: return "a required pointer is NULL";
     case GDN2_ERR_SHAPE: return "inconsistent shapes";
     case GDN2_ERR_DTYPE: return "unsupported dtype";
-    case GDN2_ERR_UNSUPPORTED_DIM: return "head dims K and V must be 64 or 128";
+    case GDN2_ERR_UNSUPPORTED_DIM: return "head dims K and V must be 64 or 128 (layer norm: at most 32768)";
     case GDN2_ERR_ALIGNMENT: return "tensor base pointers must be 16-byte aligned";
     case GDN2_ERR_WORKSPACE: return "workspace missing or too small";
     case GDN2_ERR_FLAGS: return "inconsistent flags";
@@ -171,6 +209,90 @@ int gdn2_recurrent_fwd(const gdn2_recurrent_args* a, gdn2_stream_t stream) {
     if (p && (reinterpret_cast<uintptr_t>(p) & 15)) return GDN2_ERR_ALIGNMENT;
   if (a->N == 0 || a->B * a->T == 0) return GDN2_OK;
   return recurrent_fwd(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t gdn2_linear_attn_workspace_size(const gdn2_linear_attn_args* a) {
+  if (check_linear_attn(a, false, true) != GDN2_OK) return 0;
+  return la_ws_layout(*a, nullptr, nullptr);
+}
+
+size_t gdn2_linear_attn_bwd_workspace_size(const gdn2_linear_attn_args* a) {
+  if (check_linear_attn(a, false, false) != GDN2_OK) return 0;
+  return la_bwd_ws_layout(*a, nullptr, nullptr);
+}
+
+int gdn2_linear_attn_fwd(const gdn2_linear_attn_args* a, void* workspace, size_t workspace_bytes,
+                         gdn2_stream_t stream) {
+  int st = check_linear_attn(a, true, true);
+  if (st) return st;
+  if (a->state_indices) return GDN2_ERR_FLAGS;
+  const size_t need = la_ws_layout(*a, nullptr, nullptr);
+  if (need > workspace_bytes || (need > 0 && !workspace) || misaligned(workspace)) return GDN2_ERR_WORKSPACE;
+  if (a->N == 0) return GDN2_OK;
+  LaWs ws;
+  la_ws_layout(*a, workspace, &ws);
+  return la_fwd_launch(*a, ws, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int gdn2_linear_attn_bwd(const gdn2_linear_attn_args* a, const gdn2_linear_attn_grads* gr, const void* workspace,
+                         size_t workspace_bytes, void* bwd_workspace, size_t bwd_workspace_bytes,
+                         gdn2_stream_t stream) {
+  int st = check_linear_attn(a, true, false);
+  if (st) return st;
+  if (a->state_indices || !(a->flags & GDN2_SAVE_FOR_BWD)) return GDN2_ERR_FLAGS;
+  if (!gr) return GDN2_ERR_NULL_POINTER;
+  if (a->B * a->T > 0 && (!gr->dout || !gr->dq || !gr->dk || !gr->dv)) return GDN2_ERR_NULL_POINTER;
+  if (gr->dg && a->decay == GDN2_DECAY_NONE) return GDN2_ERR_FLAGS;
+  const void* ptrs[] = {gr->dout, gr->dht, gr->dq, gr->dk, gr->dv, gr->dh0};
+  for (const void* p : ptrs)
+    if (misaligned(p)) return GDN2_ERR_ALIGNMENT;
+  const size_t need = la_ws_layout(*a, nullptr, nullptr), need_b = la_bwd_ws_layout(*a, nullptr, nullptr);
+  if (need > workspace_bytes || (need > 0 && !workspace) || misaligned(workspace)) return GDN2_ERR_WORKSPACE;
+  if (need_b > bwd_workspace_bytes || (need_b > 0 && !bwd_workspace) || misaligned(bwd_workspace))
+    return GDN2_ERR_WORKSPACE;
+  if (a->N == 0) return GDN2_OK;
+  LaWs ws;
+  la_ws_layout(*a, const_cast<void*>(workspace), &ws);
+  LaBwdWs bw;
+  la_bwd_ws_layout(*a, bwd_workspace, &bw);
+  return la_bwd_launch(*a, *gr, ws, bw, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int gdn2_linear_attn_recurrent_fwd(const gdn2_linear_attn_args* a, gdn2_stream_t stream) {
+  int st = check_linear_attn(a, true, true);
+  if (st) return st;
+  if (a->flags & GDN2_SAVE_FOR_BWD) return GDN2_ERR_FLAGS;
+  if (a->state_indices && a->num_slots < 0) return GDN2_ERR_SHAPE;
+  if (a->state_stride_in % 4 || a->state_stride_out % 4) return GDN2_ERR_ALIGNMENT;
+  if (a->N * a->HV * (a->V / 32) >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
+  if (a->N == 0) return GDN2_OK;
+  return la_recurrent_launch(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int gdn2_layer_norm_fwd(const gdn2_layer_norm_args* a, gdn2_stream_t stream) {
+  const int st = check_layer_norm(a);
+  if (st) return st;
+  if (a->rows == 0) return GDN2_OK;
+  if (!a->x || !a->y || (a->residual && !a->s) || (a->mean && !a->rstd)) return GDN2_ERR_NULL_POINTER;
+  return layer_norm_fwd_launch(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t gdn2_layer_norm_bwd_workspace_size(const gdn2_layer_norm_args* a) {
+  return check_layer_norm(a) == GDN2_OK ? layer_norm_bwd_ws(*a) : 0;
+}
+
+int gdn2_layer_norm_bwd(const gdn2_layer_norm_args* a, const gdn2_layer_norm_grads* g, void* workspace,
+                        size_t workspace_bytes, gdn2_stream_t stream) {
+  const int st = check_layer_norm(a);
+  if (st) return st;
+  if (!g) return GDN2_ERR_NULL_POINTER;
+  if (a->rows > 0 && (!a->mean || !a->rstd || !g->s || !g->dy || !(g->dx || g->dresidual)))
+    return GDN2_ERR_NULL_POINTER;
+  if (g->dweight || g->dbias) {
+    if (layer_norm_bwd_ws(*a) > workspace_bytes || !workspace || misaligned(workspace)) return GDN2_ERR_WORKSPACE;
+    if (a->dtype_weight != GDN2_BF16 && a->dtype_weight != GDN2_F32) return GDN2_ERR_DTYPE;
+  }
+  return layer_norm_bwd_launch(*a, *g, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,138 @@
+// Linear attention with a decay for each head: geometry, workspace layout and
+// the launchers behind the gdn2_linear_attn_* entry points.
+#pragma once
+
+#include "common.cuh"
+
+namespace gdn2 {
+
+constexpr int kLaChunkF32 = 64;  // tokens per chunk of the fp32 kernels
+
+// A chunk of a packed batch: its sequence (-1: past the last chunk) and its index there.
+struct LaChunk {
+  int32_t n, c;
+};
+
+struct LaGeom {
+  const int64_t* cu;
+  int64_t T, N;
+  int C;              // tokens per chunk
+  int64_t nts;        // chunks per sequence (dense)
+  const LaChunk* map;   // [NT] (packed)
+  const int32_t* first; // [N + 1] first chunk of each sequence (packed)
+
+  // first row and length of sequence n, clipped to the tensor (packed rows: B == 1)
+  GDN2_DEV void seq(int64_t n, int64_t& bos, int64_t& len) const {
+    if (cu) {
+      bos = min(max(cu[n], (int64_t)0), T);
+      len = min(max(cu[n + 1], bos), T) - bos;
+    } else {
+      bos = n * T;
+      len = T;
+    }
+  }
+  GDN2_DEV int64_t chunk0(int64_t n) const { return cu ? (int64_t)first[n] : n * nts; }
+  // chunk id -> (sequence, chunk in it); false past the last chunk
+  GDN2_DEV bool chunk(int64_t id, int64_t& n, int64_t& c) const {
+    if (cu) {
+      const LaChunk m = map[id];
+      n = m.n;
+      c = m.c;
+      return n >= 0;
+    }
+    n = id / nts;
+    c = id - n * nts;
+    return true;
+  }
+};
+
+struct LaWs {
+  LaChunk* map;     // [NT]   packed only
+  int32_t* first;   // [N+1]  packed only
+  float* total;     // [NT, HV] exp of each chunk's summed decay (fp32 kernels)
+  float* states;    // [NT, HV, K, V] fp32 (fp32 kernels)
+};
+struct LaBwdWs {
+  float* dstates;   // [NT, HV, K, V] fp32 (fp32 kernels)
+  float* dg;        // [B, T, HV] fp32, the terms of a per-head decay's gradient
+};
+
+inline int la_chunk(const gdn2_linear_attn_args&) { return kLaChunkF32; }
+
+// chunks over all sequences: exact for dense batches, an upper bound for packed
+// ones (the lengths stay on the device): sum ceil(len / C) <= T / C + N
+inline int64_t la_num_chunks(const gdn2_linear_attn_args& a) {
+  const int64_t C = la_chunk(a);
+  return a.cu_seqlens ? a.T / C + a.N : a.B * ((a.T + C - 1) / C);
+}
+
+inline size_t la_align(size_t x) { return (x + 255) & ~size_t(255); }
+
+inline size_t la_ws_layout(const gdn2_linear_attn_args& a, void* base, LaWs* out) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = la_align(off + bytes);
+    return base ? (void*)((char*)base + o) : nullptr;
+  };
+  LaWs w{};
+  const size_t NT = (size_t)la_num_chunks(a), HV = (size_t)a.HV, KV = (size_t)(a.K * a.V);
+  if (a.cu_seqlens) {
+    w.map = (LaChunk*)take(NT * sizeof(LaChunk));
+    w.first = (int32_t*)take(((size_t)a.N + 1) * 4);
+  }
+  w.total = (float*)take(NT * HV * 4);
+  w.states = (float*)take(NT * HV * KV * 4);
+  if (out) *out = w;
+  return off;
+}
+
+inline size_t la_bwd_ws_layout(const gdn2_linear_attn_args& a, void* base, LaBwdWs* out) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = la_align(off + bytes);
+    return base ? (void*)((char*)base + o) : nullptr;
+  };
+  LaBwdWs w{};
+  const size_t NT = (size_t)la_num_chunks(a), HV = (size_t)a.HV, KV = (size_t)(a.K * a.V);
+  w.dstates = (float*)take(NT * HV * KV * 4);
+  if (a.decay == GDN2_DECAY_HEAD) w.dg = (float*)take((size_t)(a.B * a.T) * HV * 4);
+  if (out) *out = w;
+  return off;
+}
+
+inline LaGeom la_geom(const gdn2_linear_attn_args& a, const LaWs& ws) {
+  const int C = la_chunk(a);
+  return LaGeom{a.cu_seqlens, a.T, a.N, C, (a.T + C - 1) / C, ws.map, ws.first};
+}
+
+// The log-decay of one token.  Values below -1e5 (and -inf) count as -1e5:
+// exp of it is zero in fp32 and sums of it stay exact to 1e-10 in fp64, so
+// differences of running sums never become inf - inf.  NaN stays NaN.
+struct LaDecay {
+  const void* g;
+  int64_t sb, st, sh;
+  int kind, dtype;
+  GDN2_DEV double at(int64_t b, int64_t t, int64_t hv) const {
+    if (kind == GDN2_DECAY_NONE) return 0.0;
+    const int64_t i = kind == GDN2_DECAY_HEAD ? hv * sh : b * sb + t * st + hv * sh;
+    const float x = dtype == GDN2_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i])
+                                       : static_cast<const float*>(g)[i];
+    return x < -1e5f ? -1e5 : (double)x;
+  }
+};
+inline LaDecay la_decay(const gdn2_linear_attn_args& a) {
+  return LaDecay{a.g, a.g_stride[0], a.g_stride[1], a.g_stride[2], a.decay, a.dtype_g};
+}
+
+int la_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s);
+int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
+                         const LaBwdWs& bw, cudaStream_t s);
+int la_recurrent_launch(const gdn2_linear_attn_args& a, cudaStream_t s);
+
+int layer_norm_fwd_launch(const gdn2_layer_norm_args& a, cudaStream_t s);
+int layer_norm_bwd_launch(const gdn2_layer_norm_args& a, const gdn2_layer_norm_grads& g, void* ws, cudaStream_t s);
+size_t layer_norm_bwd_ws(const gdn2_layer_norm_args& a);
+
+}  // namespace gdn2

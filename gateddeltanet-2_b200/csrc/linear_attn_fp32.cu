@@ -1,0 +1,666 @@
+// Linear attention with a decay for each head, fp32 arithmetic throughout
+// (the fp32 path).  With G the running sum of g inside a chunk of C = 64
+// tokens and S, dS' the state entering and the state cotangent leaving it:
+//     P_ij = e^{G_i - G_j} (q_i . k_j),  E_ij = e^{G_i - G_j} (do_i . v_j)   (i >= j)
+//     o  = scale (P v + e^G q S)          S' = e^{G_C} S + sum_j e^{G_C - G_j} k_j v_j^T
+//     dq = scale (E k + e^G do S^T)       dk = scale E^T q + e^{G_C - G} v dS'^T
+//     dv = scale P^T do + e^{G_C - G} k dS'
+//     dS = e^{G_C} dS' + scale sum_i e^{G_i} q_i do_i^T
+//     dg_t = sum_{i>=t} (sum_{j<i} M_ij + q_i . dq_i^inter) - sum_{j>=t} sum_{i>j} M_ij
+//            + sum_{j<t} k_j . dk_j^inter + e^{G_C} <S, dS'>,   M = scale P E / e^{G_i - G_j}
+// (the diagonal of M cancels and is left out, so a token that no decay acts
+// on gets an exact zero).  Three steps each way: every chunk's own state term,
+// a running sum of those over the chunks of a sequence, and every chunk's
+// outputs.  Running sums of g and their differences are held in fp64: their
+// exponentials then carry only their own rounding, however long or strong the decay.
+#include "linear_attn.cuh"
+#include "profile.cuh"
+
+namespace gdn2 {
+namespace {
+
+constexpr int kC = kLaChunkF32;
+constexpr int kThreads = 256;
+constexpr int kLdP = kC + 1;
+
+// acc[r][c] += sum_k A(4 ty + r, k) B(k, tx + 16 c); strides in elements.
+// A row is shared by the 16 threads of a half warp (broadcast); consecutive tx
+// read consecutive columns, or rows of odd length (no bank conflicts either way).
+template <int NJ>
+GDN2_DEV void tile_mm(float (&acc)[4][NJ], const float* A, int sai, int sak, const float* B, int sbk, int sbj,
+                      int kdim) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  A += 4 * ty * sai;
+  B += tx * sbj;
+#pragma unroll 4
+  for (int k = 0; k < kdim; ++k) {
+    float x[4], y[NJ];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = A[r * sai + k * sak];
+#pragma unroll
+    for (int c = 0; c < NJ; ++c) y[c] = B[k * sbk + 16 * c * sbj];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < NJ; ++c) acc[r][c] = fmaf(x[r], y[c], acc[r][c]);
+  }
+}
+
+template <int NJ>
+GDN2_DEV void zero(float (&acc)[4][NJ]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < NJ; ++c) acc[r][c] = 0.f;
+}
+
+// L rows of D elements (row stride st) into a padded fp32 tile, zero rows after them
+template <typename T, int D>
+GDN2_DEV void load_rows(float* dst, const T* src, int64_t st, int L) {
+  for (int i = threadIdx.x; i < kC * D; i += kThreads) {
+    const int r = i / D, c = i % D;
+    dst[r * (D + 1) + c] = r < L ? to_f(src[r * st + c]) : 0.f;
+  }
+}
+
+// running sums of the chunk's log-decays (warp 0; two tokens per lane)
+GDN2_DEV void chunk_sums(double* G, const LaDecay& d, int64_t b, int64_t t0, int64_t hv, int L) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    const double x0 = 2 * lane < L ? d.at(b, t0 + 2 * lane, hv) : 0.0;
+    const double x1 = 2 * lane + 1 < L ? d.at(b, t0 + 2 * lane + 1, hv) : 0.0;
+    double s = x0 + x1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    const double before = __shfl_up_sync(0xffffffffu, s, 1);
+    G[2 * lane] = (lane ? before : 0.0) + x0;
+    G[2 * lane + 1] = s;
+  }
+}
+
+struct Where {
+  int64_t n, c, b, t0, tok0;  // sequence, chunk in it, batch row, first token in that row, and over all rows
+  int L;
+};
+GDN2_DEV bool locate(const LaGeom& geo, int64_t id, Where& w) {
+  if (!geo.chunk(id, w.n, w.c)) return false;
+  int64_t bos, len;
+  geo.seq(w.n, bos, len);
+  const int64_t left = len - w.c * kC;
+  w.L = (int)min(left, (int64_t)kC);
+  w.tok0 = bos + w.c * kC;
+  w.b = geo.cu ? 0 : w.n;
+  w.t0 = geo.cu ? w.tok0 : w.c * kC;
+  return w.L > 0;
+}
+
+// One chunk's own term of the state recurrence, sum_t w_t x_t y_t^T: forward
+// x = k, y = v, w_t = e^{G_C - G_t}; backward x = q, y = do, w_t = scale e^{G_t}.
+// 8 x 8 (or smaller) outputs per thread.
+template <typename T, int K, int V, bool kBack>
+__global__ void __launch_bounds__(kThreads) la_state_kernel(const T* x, int64_t xb, int64_t xt, int64_t xh, const T* y,
+                                                            int64_t yb, int64_t yt, int64_t yh, LaDecay dec,
+                                                            LaGeom geo, int HV, int group, float scale, float* states,
+                                                            float* total) {
+  extern __shared__ float sm[];
+  float* X = sm;
+  float* Y = X + kC * (K + 1);
+  __shared__ double G[kC];
+  Where w;
+  const int hv = blockIdx.y;
+  if (!locate(geo, blockIdx.x, w)) return;
+  load_rows<T, K>(X, x + w.b * xb + w.t0 * xt + (hv / group) * xh, xt, w.L);
+  load_rows<T, V>(Y, y + w.b * yb + w.t0 * yt + hv * yh, yt, w.L);
+  chunk_sums(G, dec, w.b, w.t0, hv, w.L);
+  __syncthreads();
+  if (threadIdx.x == 0 && total) total[(int64_t)blockIdx.x * HV + hv] = expf((float)G[kC - 1]);
+  for (int i = threadIdx.x; i < kC * V; i += kThreads) {
+    const int t = i / V;
+    const float f = kBack ? scale * expf((float)G[t]) : expf((float)(G[kC - 1] - G[t]));
+    if (t < w.L) Y[t * (V + 1) + i % V] *= f;
+  }
+  __syncthreads();
+  constexpr int R = K / 16, NJ = V / 16;
+  float acc[R][NJ];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < NJ; ++c) acc[r][c] = 0.f;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  for (int t = 0; t < w.L; ++t) {
+    float a[R], bb[NJ];
+#pragma unroll
+    for (int r = 0; r < R; ++r) a[r] = X[t * (K + 1) + ty + 16 * r];
+#pragma unroll
+    for (int c = 0; c < NJ; ++c) bb[c] = Y[t * (V + 1) + tx + 16 * c];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int c = 0; c < NJ; ++c) acc[r][c] = fmaf(a[r], bb[c], acc[r][c]);
+  }
+  float* dst = states + ((int64_t)blockIdx.x * HV + hv) * K * V;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < NJ; ++c) dst[(ty + 16 * r) * V + tx + 16 * c] = acc[r][c];
+}
+
+// The running sum over a sequence's chunks, in place: states[c] becomes the
+// state entering chunk c (forward), or the cotangent leaving it (backward, from
+// the last chunk).  Four elements per thread; the loads of kAhead chunks are in flight.
+template <bool kBack>
+__global__ void __launch_bounds__(128) la_prefix_kernel(float* states, const float* total, const float* init, float* fin,
+                                                        LaGeom geo, int HV, int64_t KV) {
+  constexpr int kAhead = 8;
+  const int64_t nh = blockIdx.x, n = nh / HV, hv = nh % HV;
+  const int64_t e = ((int64_t)blockIdx.y * 128 + threadIdx.x) * 4;
+  if (e >= KV) return;
+  int64_t bos, len;
+  geo.seq(n, bos, len);
+  const int64_t nch = (len + kC - 1) / kC, c0 = geo.chunk0(n);
+  float4 s = init ? *reinterpret_cast<const float4*>(init + nh * KV + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int64_t i0 = 0; i0 < nch; i0 += kAhead) {
+    float4 add[kAhead];
+    float f[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i0 + i < nch) {
+        const int64_t c = c0 + (kBack ? nch - 1 - (i0 + i) : i0 + i);
+        add[i] = *reinterpret_cast<const float4*>(states + (c * HV + hv) * KV + e);
+        f[i] = total[c * HV + hv];
+      }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i0 + i < nch) {
+        const int64_t c = c0 + (kBack ? nch - 1 - (i0 + i) : i0 + i);
+        *reinterpret_cast<float4*>(states + (c * HV + hv) * KV + e) = s;
+        s.x = fmaf(s.x, f[i], add[i].x);
+        s.y = fmaf(s.y, f[i], add[i].y);
+        s.z = fmaf(s.z, f[i], add[i].z);
+        s.w = fmaf(s.w, f[i], add[i].w);
+      }
+  }
+  if (fin) *reinterpret_cast<float4*>(fin + nh * KV + e) = s;
+}
+
+template <typename T, int K, int V>
+__global__ void __launch_bounds__(kThreads) la_out_kernel(gdn2_linear_attn_args a, LaDecay dec, LaGeom geo,
+                                                          const float* states) {
+  extern __shared__ float sm[];
+  float* Q = sm;
+  float* Kt = Q + kC * (K + 1);
+  float* Vt = Kt + kC * (K + 1);
+  float* P = Vt + kC * (V + 1);
+  float* S = P + kC * kLdP;  // 64 rows of the state at a time
+  __shared__ double G[kC];
+  Where w;
+  const int64_t HV = a.HV, hv = blockIdx.y, h = hv / (HV / a.H);
+  if (!locate(geo, blockIdx.x, w)) return;
+  load_rows<T, K>(Q, static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.t0 * a.q_stride[1] + h * a.q_stride[2],
+                  a.q_stride[1], w.L);
+  load_rows<T, K>(Kt, static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.t0 * a.k_stride[1] + h * a.k_stride[2],
+                  a.k_stride[1], w.L);
+  load_rows<T, V>(Vt, static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.t0 * a.v_stride[1] + hv * a.v_stride[2],
+                  a.v_stride[1], w.L);
+  chunk_sums(G, dec, w.b, w.t0, hv, w.L);
+  __syncthreads();
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  {
+    float p[4][4];
+    zero(p);
+    tile_mm(p, Q, K + 1, 1, Kt, 1, K + 1, K);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int i = 4 * ty + r, j = tx + 16 * c;
+        P[i * kLdP + j] = i >= j ? p[r][c] * expf((float)(G[i] - G[j])) : 0.f;
+      }
+  }
+  constexpr int NJ = V / 16;
+  float o[4][NJ];
+  zero(o);
+  const float* st = states + ((int64_t)blockIdx.x * HV + hv) * K * V;
+  for (int k0 = 0; k0 < K; k0 += 64) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * V; i += kThreads) S[(i / V) * (V + 1) + i % V] = st[k0 * V + i];
+    __syncthreads();
+    tile_mm(o, Q + k0, K + 1, 1, S, V + 1, 1, 64);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float f = expf((float)G[4 * ty + r]);
+#pragma unroll
+    for (int c = 0; c < NJ; ++c) o[r][c] *= f;
+  }
+  tile_mm(o, P, kLdP, 1, Vt, V + 1, 1, kC);
+  T* out = static_cast<T*>(a.o);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < NJ; ++c)
+      if (4 * ty + r < w.L)
+        out[((w.tok0 + 4 * ty + r) * HV + hv) * V + tx + 16 * c] = from_f<T>(a.scale * o[r][c]);
+}
+
+// sum over the 16 threads tx of a row group; every one of them gets it
+GDN2_DEV float row_sum(float x) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// One CTA per (chunk, key head): the value heads of the group one after the
+// other, their shares of dq and dk added up in registers.
+template <typename T, int K, int V>
+__global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args a, gdn2_linear_attn_grads gr,
+                                                          LaDecay dec, LaGeom geo, const float* states,
+                                                          const float* dstates, float* dgf) {
+  extern __shared__ float sm[];
+  float* Q = sm;
+  float* Kt = Q + kC * (K + 1);
+  float* Vt = Kt + kC * (K + 1);
+  float* D = Vt + kC * (V + 1);
+  float* P = D + kC * (V + 1);
+  float* E = P + kC * kLdP;
+  float* S = E + kC * kLdP;  // half of a state, [64][128 + 1] or [128][64 + 1]
+  __shared__ double G[kC];
+  __shared__ float colw[8][kC], rows[kC], qint[kC], kint[kC], wsum[8];
+  Where w;
+  const int64_t H = a.H, HV = a.HV, h = blockIdx.y;
+  const int group = (int)(HV / H);
+  if (!locate(geo, blockIdx.x, w)) return;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int NK = K / 16, NV = V / 16;
+  const bool want_dg = gr.dg != nullptr;
+  float dq[4][NK], dk[4][NK];
+  zero(dq);
+  zero(dk);
+  load_rows<T, K>(Q, static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.t0 * a.q_stride[1] + h * a.q_stride[2],
+                  a.q_stride[1], w.L);
+  load_rows<T, K>(Kt, static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.t0 * a.k_stride[1] + h * a.k_stride[2],
+                  a.k_stride[1], w.L);
+  for (int j = 0; j < group; ++j) {
+    const int64_t hv = h * group + j;
+    __syncthreads();
+    load_rows<T, V>(Vt, static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.t0 * a.v_stride[1] + hv * a.v_stride[2],
+                    a.v_stride[1], w.L);
+    load_rows<T, V>(D, static_cast<const T*>(gr.dout) + (w.tok0 * HV + hv) * V, HV * V, w.L);
+    chunk_sums(G, dec, w.b, w.t0, hv, w.L);
+    __syncthreads();
+    const float* st = states + ((int64_t)blockIdx.x * HV + hv) * K * V;
+    const float* dst = dstates + ((int64_t)blockIdx.x * HV + hv) * K * V;
+    const double GC = G[kC - 1];
+    {
+      float p[4][4], e[4][4], col[4] = {0.f, 0.f, 0.f, 0.f};
+      zero(p);
+      zero(e);
+      tile_mm(p, Q, K + 1, 1, Kt, 1, K + 1, K);
+      tile_mm(e, D, V + 1, 1, Vt, 1, V + 1, V);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float row = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int i = 4 * ty + r, jj = tx + 16 * c;
+          const float f = i >= jj ? a.scale * expf((float)(G[i] - G[jj])) : 0.f;
+          P[i * kLdP + jj] = i >= jj ? p[r][c] * f : 0.f;
+          E[i * kLdP + jj] = i >= jj ? e[r][c] * f : 0.f;
+          if (i > jj) {
+            const float m = p[r][c] * e[r][c] * f;
+            row += m;
+            col[c] += m;
+          }
+        }
+        if (want_dg) {
+          row = row_sum(row);
+          if (tx == 0) rows[4 * ty + r] = row;
+        }
+      }
+      if (want_dg) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x = col[c] + __shfl_xor_sync(0xffffffffu, col[c], 16);
+          if (lane < 16) colw[warp][tx + 16 * c] = x;
+        }
+      }
+    }
+    {  // dv = e^{G_C - G} k dS' + P^T do
+      float acc[4][NV];
+      zero(acc);
+      for (int k0 = 0; k0 < K; k0 += 64) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 64 * V; i += kThreads) S[(i / V) * (V + 1) + i % V] = dst[k0 * V + i];
+        __syncthreads();
+        tile_mm(acc, Kt + k0, K + 1, 1, S, V + 1, 1, 64);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float f = expf((float)(GC - G[4 * ty + r]));
+#pragma unroll
+        for (int c = 0; c < NV; ++c) acc[r][c] *= f;
+      }
+      tile_mm(acc, P, 1, kLdP, D, V + 1, 1, kC);
+      T* out = static_cast<T*>(gr.dv);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+          if (4 * ty + r < w.L) out[((w.tok0 + 4 * ty + r) * HV + hv) * V + tx + 16 * c] = from_f<T>(acc[r][c]);
+    }
+    {  // dq += scale e^G do S^T + E k
+      float acc[4][NK];
+      zero(acc);
+      for (int v0 = 0; v0 < V; v0 += 64) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < K * 64; i += kThreads) S[(i / 64) * 65 + i % 64] = st[(i / 64) * V + v0 + i % 64];
+        __syncthreads();
+        tile_mm(acc, D + v0, V + 1, 1, S, 1, 65, 64);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float f = a.scale * expf((float)G[4 * ty + r]);
+        float x = 0.f;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+          acc[r][c] *= f;
+          x = fmaf(acc[r][c], Q[(4 * ty + r) * (K + 1) + tx + 16 * c], x);
+        }
+        if (want_dg) {
+          x = row_sum(x);
+          if (tx == 0) qint[4 * ty + r] = x;
+        }
+      }
+      tile_mm(acc, E, kLdP, 1, Kt, K + 1, 1, kC);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < NK; ++c) dq[r][c] += acc[r][c];
+    }
+    {  // dk += e^{G_C - G} v dS'^T + E^T q
+      float acc[4][NK];
+      zero(acc);
+      for (int v0 = 0; v0 < V; v0 += 64) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < K * 64; i += kThreads) S[(i / 64) * 65 + i % 64] = dst[(i / 64) * V + v0 + i % 64];
+        __syncthreads();
+        tile_mm(acc, Vt + v0, V + 1, 1, S, 1, 65, 64);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float f = expf((float)(GC - G[4 * ty + r]));
+        float x = 0.f;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+          acc[r][c] *= f;
+          x = fmaf(acc[r][c], Kt[(4 * ty + r) * (K + 1) + tx + 16 * c], x);
+        }
+        if (want_dg) {
+          x = row_sum(x);
+          if (tx == 0) kint[4 * ty + r] = x;
+        }
+      }
+      tile_mm(acc, E, 1, kLdP, Q, K + 1, 1, kC);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < NK; ++c) dk[r][c] += acc[r][c];
+    }
+    if (want_dg) {
+      float x = 0.f;
+      for (int i = threadIdx.x; i < K * V; i += kThreads) x = fmaf(st[i], dst[i], x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      if (lane == 0) wsum[warp] = x;
+      __syncthreads();
+      if (threadIdx.x < kC) {
+        float x0 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x0 += wsum[i];
+        const int t = threadIdx.x;
+        float d = expf((float)GC) * x0;
+        for (int i = t; i < kC; ++i) {
+          float cs = 0.f;
+#pragma unroll
+          for (int ww = 0; ww < 8; ++ww) cs += colw[ww][i];
+          d += rows[i] + qint[i] - cs;
+        }
+        for (int i = 0; i < t; ++i) d += kint[i];
+        if (t < w.L) {
+          const int64_t at = (w.tok0 + t) * HV + hv;
+          if (dgf) dgf[at] = d;
+          else if (a.dtype_g == GDN2_BF16) static_cast<__nv_bfloat16*>(gr.dg)[at] = __float2bfloat16_rn(d);
+          else static_cast<float*>(gr.dg)[at] = d;
+        }
+      }
+    }
+  }
+  T* oq = static_cast<T*>(gr.dq);
+  T* ok = static_cast<T*>(gr.dk);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+      if (4 * ty + r < w.L) {
+        const int64_t at = ((w.tok0 + 4 * ty + r) * H + h) * K + tx + 16 * c;
+        oq[at] = from_f<T>(dq[r][c]);
+        ok[at] = from_f<T>(dk[r][c]);
+      }
+}
+
+// gradient of one decay per head: the sum of its tokens' (fixed order)
+__global__ void __launch_bounds__(256) la_head_sum_kernel(const float* dg, int64_t tokens, int HV, void* out, int dtype,
+                                                          LaGeom geo) {
+  __shared__ double part[8];
+  const int hv = blockIdx.x;
+  double s = 0.0;
+  for (int64_t n = 0; n < geo.N; ++n) {
+    int64_t bos, len;
+    geo.seq(n, bos, len);
+    for (int64_t t = threadIdx.x; t < len; t += 256) s += dg[(bos + t) * HV + hv];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int i = 0; i < 8; ++i) s += part[i];
+    if (dtype == GDN2_BF16) static_cast<__nv_bfloat16*>(out)[hv] = __float2bfloat16_rn((float)s);
+    else static_cast<float*>(out)[hv] = (float)s;
+  }
+}
+
+// (sequence, chunk) of every chunk id of a packed batch, and each sequence's
+// first chunk: one CTA walks the lengths 1024 at a time with a block prefix sum.
+__global__ void __launch_bounds__(1024) la_chunk_map_kernel(LaGeom geo, LaChunk* map, int32_t* first, int64_t NT) {
+  __shared__ int64_t warp_sum[32];
+  __shared__ int64_t carry;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) carry = 0;
+  __syncthreads();
+  for (int64_t n0 = 0; n0 < geo.N; n0 += 1024) {
+    const int64_t n = n0 + tid;
+    int64_t bos = 0, len = 0;
+    if (n < geo.N) geo.seq(n, bos, len);
+    const int64_t nch = (len + geo.C - 1) / geo.C;
+    int64_t s = nch;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    int64_t base = carry;
+    for (int i = 0; i < warp; ++i) base += warp_sum[i];
+    if (n < geo.N) first[n] = (int32_t)min(base + s - nch, NT);
+    __syncthreads();
+    if (tid == 1023) carry = base + s;
+    __syncthreads();
+  }
+  const int64_t all = min(carry, NT);
+  if (tid == 0) first[geo.N] = (int32_t)all;
+  __syncthreads();
+  for (int64_t id = tid; id < NT; id += 1024) {
+    LaChunk m{-1, 0};
+    if (id < all) {  // the last sequence whose first chunk is <= id
+      int64_t lo = 0, hi = geo.N;
+      while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        if (first[mid] <= id) lo = mid;
+        else hi = mid;
+      }
+      m.n = (int32_t)lo;
+      m.c = (int32_t)(id - first[lo]);
+    }
+    map[id] = m;
+  }
+}
+
+// Rows of packed tensors that lie in no sequence (before the first offset,
+// after the last) get zeros.  Offsets that cover the row, the usual case, leave nothing to do.
+struct LaRows {
+  void* p[4];
+  int64_t bytes[4];  // of one row
+};
+__global__ void __launch_bounds__(256) la_zero_outside_kernel(LaRows r, LaGeom geo) {
+  int64_t b0, l0, b1, l1;
+  geo.seq(0, b0, l0);
+  geo.seq(geo.N - 1, b1, l1);
+  const int64_t end = b1 + l1, rows = b0 + (geo.T - end);
+  if (rows <= 0) return;
+  for (int i = 0; i < 4; ++i) {
+    if (!r.p[i]) continue;
+    const int64_t units = r.bytes[i] / 2;  // every row is a whole number of 2-byte units
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < rows * units; x += (int64_t)gridDim.x * 256) {
+      const int64_t k = x / units, row = k < b0 ? k : end + (k - b0);
+      static_cast<uint16_t*>(r.p[i])[row * units + x % units] = 0;
+    }
+  }
+}
+
+template <typename F>
+int set_smem(F f, size_t bytes) {
+  GDN2_CUDA_TRY(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return 0;
+}
+
+template <typename T, int K, int V>
+int fwd(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
+  const LaGeom geo = la_geom(a, ws);
+  const LaDecay dec = la_decay(a);
+  const int64_t NT = la_num_chunks(a);
+  const int HV = (int)a.HV, group = (int)(a.HV / a.H);
+  const float* h0 = (a.flags & GDN2_HAS_H0) ? a.h0 : nullptr;
+  float* ht = (a.flags & GDN2_STORE_FINAL) ? a.ht : nullptr;
+  ProfScope ps(kKLinAttnFp32, s);
+  if (NT > 0) {
+    const size_t sm = kC * (K + 1 + V + 1) * 4;
+    if (int st = set_smem(la_state_kernel<T, K, V, false>, sm)) return st;
+    la_state_kernel<T, K, V, false><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
+        static_cast<const T*>(a.k), a.k_stride[0], a.k_stride[1], a.k_stride[2], static_cast<const T*>(a.v),
+        a.v_stride[0], a.v_stride[1], a.v_stride[2], dec, geo, HV, group, 1.f, ws.states, ws.total);
+    GDN2_LAUNCH_CHECK();
+  }
+  la_prefix_kernel<false><<<dim3((unsigned)(a.N * HV), (K * V + 511) / 512), 128, 0, s>>>(ws.states, ws.total, h0, ht,
+                                                                                          geo, HV, K * V);
+  GDN2_LAUNCH_CHECK();
+  if (NT > 0) {
+    const size_t sm = (2 * kC * (K + 1) + kC * (V + 1) + kC * kLdP + 64 * (V + 1)) * 4;
+    if (int st = set_smem(la_out_kernel<T, K, V>, sm)) return st;
+    la_out_kernel<T, K, V><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(a, dec, geo, ws.states);
+    GDN2_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+template <typename T, int K, int V>
+int bwd(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws, const LaBwdWs& bw,
+        cudaStream_t s) {
+  const LaGeom geo = la_geom(a, ws);
+  const LaDecay dec = la_decay(a);
+  const int64_t NT = la_num_chunks(a);
+  const int HV = (int)a.HV, group = (int)(a.HV / a.H);
+  ProfScope ps(kKLinAttnFp32, s);
+  if (NT > 0) {
+    const size_t sm = kC * (K + 1 + V + 1) * 4;
+    if (int st = set_smem(la_state_kernel<T, K, V, true>, sm)) return st;
+    la_state_kernel<T, K, V, true><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
+        static_cast<const T*>(a.q), a.q_stride[0], a.q_stride[1], a.q_stride[2], static_cast<const T*>(gr.dout),
+        a.T * HV * V, (int64_t)HV * V, V, dec, geo, HV, group, a.scale, bw.dstates, nullptr);
+    GDN2_LAUNCH_CHECK();
+  }
+  la_prefix_kernel<true><<<dim3((unsigned)(a.N * HV), (K * V + 511) / 512), 128, 0, s>>>(
+      bw.dstates, ws.total, gr.dht, gr.dh0, geo, HV, K * V);
+  GDN2_LAUNCH_CHECK();
+  if (NT > 0) {
+    constexpr int half = 64 * (V + 1) > K * 65 ? 64 * (V + 1) : K * 65;
+    const size_t sm = (2 * kC * (K + 1) + 2 * kC * (V + 1) + 2 * kC * kLdP + half) * 4;
+    if (int st = set_smem(la_bwd_kernel<T, K, V>, sm)) return st;
+    la_bwd_kernel<T, K, V><<<dim3((unsigned)NT, (unsigned)a.H), kThreads, sm, s>>>(
+        a, gr, dec, geo, ws.states, bw.dstates, a.decay == GDN2_DECAY_HEAD ? bw.dg : nullptr);
+    GDN2_LAUNCH_CHECK();
+  }
+  if (gr.dg && a.decay == GDN2_DECAY_HEAD) {
+    la_head_sum_kernel<<<HV, 256, 0, s>>>(bw.dg, a.B * a.T, HV, gr.dg, a.dtype_g, geo);
+    GDN2_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+template <typename T, typename F>
+int by_dims(const gdn2_linear_attn_args& a, F f) {
+  if (a.K == 128) return a.V == 128 ? f.template operator()<T, 128, 128>() : f.template operator()<T, 128, 64>();
+  return a.V == 128 ? f.template operator()<T, 64, 128>() : f.template operator()<T, 64, 64>();
+}
+
+struct FwdCall {
+  const gdn2_linear_attn_args& a;
+  const LaWs& ws;
+  cudaStream_t s;
+  template <typename T, int K, int V>
+  int operator()() const { return fwd<T, K, V>(a, ws, s); }
+};
+struct BwdCall {
+  const gdn2_linear_attn_args& a;
+  const gdn2_linear_attn_grads& gr;
+  const LaWs& ws;
+  const LaBwdWs& bw;
+  cudaStream_t s;
+  template <typename T, int K, int V>
+  int operator()() const { return bwd<T, K, V>(a, gr, ws, bw, s); }
+};
+
+}  // namespace
+
+int la_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
+  if (a.cu_seqlens) {
+    la_chunk_map_kernel<<<1, 1024, 0, s>>>(la_geom(a, ws), ws.map, ws.first, la_num_chunks(a));
+    GDN2_LAUNCH_CHECK();
+    const int64_t e = a.dtype == GDN2_BF16 ? 2 : 4;
+    la_zero_outside_kernel<<<32, 256, 0, s>>>(LaRows{{a.o}, {a.HV * a.V * e}}, la_geom(a, ws));
+    GDN2_LAUNCH_CHECK();
+  }
+  const FwdCall f{a, ws, s};
+  return a.dtype == GDN2_F32 ? by_dims<float>(a, f) : by_dims<__nv_bfloat16>(a, f);
+}
+
+int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
+                  const LaBwdWs& bw, cudaStream_t s) {
+  if (a.cu_seqlens) {
+    const int64_t e = a.dtype == GDN2_BF16 ? 2 : 4, eg = a.dtype_g == GDN2_BF16 ? 2 : 4;
+    const bool token = a.decay == GDN2_DECAY_TOKEN;
+    la_zero_outside_kernel<<<32, 256, 0, s>>>(LaRows{{gr.dq, gr.dk, gr.dv, token ? gr.dg : nullptr},
+                                                     {a.H * a.K * e, a.H * a.K * e, a.HV * a.V * e, a.HV * eg}},
+                                              la_geom(a, ws));
+    GDN2_LAUNCH_CHECK();
+  }
+  const BwdCall f{a, gr, ws, bw, s};
+  return a.dtype == GDN2_F32 ? by_dims<float>(a, f) : by_dims<__nv_bfloat16>(a, f);
+}
+
+}  // namespace gdn2

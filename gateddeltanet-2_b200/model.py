@@ -11,7 +11,11 @@ fused per-head qkv projection, RoPE on q and k in fp32, flash attention with
 window ``(local_window - 1, 0)``) and ``SwiGLU`` (``:401-412``), so a
 reference state dict for the same shape loads unchanged.
 
-Only the GDN2 mixers are this build's kernels.  Attention runs flash_attn's
+``HybridConfig.mixer = "linear"`` puts ``LinearAttention`` (a decay for each
+head, no erase term) in the place of ``GatedDeltaNet2``, ``norm = "layer"``
+this package's ``LayerNorm`` in the place of RMSNorm, its residual add fused.
+
+Only the GDN2 and linear-attention mixers and the layer norm are this build's kernels.  Attention runs flash_attn's
 library kernel (``flash_attn_func`` with a window, as the reference does);
 the GEMMs run cuBLAS; RMSNorm, RoPE, SwiGLU's gate and the loss are torch.
 """
@@ -26,6 +30,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .layer import GatedDeltaNet2
+from .layer_norm import LayerNorm
+from .linear_layer import LinearAttention
 
 
 @dataclass
@@ -45,6 +51,14 @@ class HybridConfig:
     block_size: int = 4096
     rope_base: int = 10000
     mamba_init: bool = True
+    mixer: str = "gdn2"  # of every gdn2_per_layer-th block: "gdn2", or "linear" (LinearAttention)
+    norm: str = "rms"    # of the blocks and before the head: "rms", or "layer" (LayerNorm)
+
+    def __post_init__(self):
+        if self.mixer not in ("gdn2", "linear"):
+            raise ValueError(f"mixer must be 'gdn2' or 'linear', got {self.mixer!r}")
+        if self.norm not in ("rms", "layer"):
+            raise ValueError(f"norm must be 'rms' or 'layer', got {self.norm!r}")
 
     @property
     def head_size(self) -> int:
@@ -66,6 +80,11 @@ class RMSNorm(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return F.rms_norm(x, (x.shape[-1],), self.weight, self.eps)
+
+
+def _norm(config: HybridConfig) -> nn.Module:
+    cls = LayerNorm if config.norm == "layer" else RMSNorm
+    return cls(config.n_embd, eps=config.norm_eps)
 
 
 def build_rope_cache(seq_len: int, n_elem: int, device, base: int = 10000):
@@ -132,19 +151,23 @@ class Block(nn.Module):
 
     def __init__(self, config: HybridConfig, layer_idx: int, gdn2_cls=None):
         super().__init__()
-        self.norm_1 = RMSNorm(config.n_embd, eps=config.norm_eps)
+        self.norm_1 = _norm(config)
         self.use_gdn2 = config.gdn2_per_layer > 0 and layer_idx % config.gdn2_per_layer == 0
         if self.use_gdn2:
-            self.attn = (gdn2_cls or GatedDeltaNet2)(hidden_size=config.n_embd, head_dim=config.head_size,
-                                                     num_heads=config.n_head, layer_idx=layer_idx)
+            cls = gdn2_cls or (LinearAttention if config.mixer == "linear" else GatedDeltaNet2)
+            self.attn = cls(hidden_size=config.n_embd, head_dim=config.head_size, num_heads=config.n_head,
+                            layer_idx=layer_idx)
         else:
             self.attn = CausalSelfAttention(config)
-        self.norm_2 = RMSNorm(config.n_embd, eps=config.norm_eps)
+        self.norm_2 = _norm(config)
         self.mlp = LLaMAMLP(config)
 
     def forward(self, x: torch.Tensor, rope) -> torch.Tensor:
         n_1 = self.norm_1(x)
         h = self.attn(n_1)[0] if self.use_gdn2 else self.attn(n_1, rope)
+        if isinstance(self.norm_2, LayerNorm):  # the residual add and the norm in one pass
+            n_2, x = self.norm_2(h, residual=x)
+            return x + self.mlp(n_2)
         x = x + h
         return x + self.mlp(self.norm_2(x))
 
@@ -161,7 +184,7 @@ class GPT(nn.Module):
         self.transformer = nn.ModuleDict(dict(
             wte=nn.Embedding(config.padded_vocab_size, config.n_embd),
             h=nn.ModuleList(Block(config, i, gdn2_cls) for i in range(config.n_layer)),
-            ln_f=RMSNorm(config.n_embd, eps=config.norm_eps),
+            ln_f=_norm(config),
         ))
         self.rope_cache = None
 

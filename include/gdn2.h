@@ -334,6 +334,119 @@ int gdn2_norm_gate_bwd(const void* dy, const void* x, const void* gate, const fl
                        void* workspace, size_t workspace_bytes, gdn2_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
+/* linear attention with a decay for each head                               */
+/* ------------------------------------------------------------------------- */
+/*
+ * The state recurrence without the delta rule's erase term, and with one decay
+ * per value head instead of one per channel:
+ *     S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t
+ * q, k: [B, T, H, K]; v, o: [B, T, HV, V] with HV a multiple of H (value head
+ * hv reads key head hv / (HV / H)); K, V in {64, 128}.  q, k and v may be
+ * strided views (for example of one projection's output): the innermost
+ * dimension is contiguous, base addresses and the other strides are multiples
+ * of 16 bytes.  g: no decay, one value per head, or one per token and head
+ * (natural log; -inf forgets the state entirely).  Packed sequences as in
+ * gdn2_chunk_fwd; spans outside [0, T) are clipped.
+ * A token whose mask or length leaves a sequence empty contributes nothing:
+ * its final state is its initial state.
+ */
+enum gdn2_decay { GDN2_DECAY_NONE = 0, GDN2_DECAY_HEAD = 1, GDN2_DECAY_TOKEN = 2 };
+
+typedef struct gdn2_linear_attn_args {
+  int64_t B, T, H, HV, K, V;
+  int64_t N;                    /* sequences: B, or len(cu_seqlens) - 1 */
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* elements between batches, tokens, heads */
+  int64_t g_stride[3];          /* the same for g (GDN2_DECAY_TOKEN), or {0, 0, head stride} */
+  const int64_t* cu_seqlens;    /* [N+1] device, or NULL for dense [B, T] */
+  const int32_t* state_indices; /* recurrent only: [N] pool slots of h0 / ht, or NULL (slot n) */
+  int64_t num_slots;            /* with state_indices: slots of the pool; a sequence whose slot is outside
+                                   [0, num_slots) is skipped and its o rows are zero */
+  int64_t state_stride_in, state_stride_out; /* recurrent only: elements between slots of h0, ht */
+  float scale;
+  int32_t flags;                /* GDN2_HAS_H0 | GDN2_STORE_FINAL | GDN2_SAVE_FOR_BWD */
+  int32_t dtype;                /* q, k, v, o, dout, dq, dk, dv: GDN2_BF16 or GDN2_F32 */
+  int32_t dtype_g;              /* g, dg: GDN2_BF16 or GDN2_F32 */
+  int32_t decay;                /* enum gdn2_decay */
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* g;
+  const float* h0;              /* [N, HV, K, V] fp32 with GDN2_HAS_H0 */
+  float* ht;                    /* [N, HV, K, V] fp32 with GDN2_STORE_FINAL (recurrent: may alias h0) */
+  void* o;                      /* [B, T, HV, V] contiguous */
+} gdn2_linear_attn_args;
+
+typedef struct gdn2_linear_attn_grads {
+  const void* dout;             /* [B, T, HV, V] contiguous */
+  const float* dht;             /* [N, HV, K, V] cotangent of the final state, or NULL */
+  void* dq;                     /* [B, T, H, K] contiguous */
+  void* dk;                     /* [B, T, H, K] contiguous */
+  void* dv;                     /* [B, T, HV, V] contiguous */
+  void* dg;                     /* [B, T, HV] (GDN2_DECAY_TOKEN) or [HV] (GDN2_DECAY_HEAD) in dtype_g, or NULL */
+  float* dh0;                   /* [N, HV, K, V], or NULL */
+} gdn2_linear_attn_grads;
+
+/* Chunkwise forward (prompts, training).  With GDN2_SAVE_FOR_BWD the workspace
+ * keeps the states entering the chunks, which the backward reads; without it
+ * the workspace is scratch. */
+size_t gdn2_linear_attn_workspace_size(const gdn2_linear_attn_args* a);
+int gdn2_linear_attn_fwd(const gdn2_linear_attn_args* a, void* workspace, size_t workspace_bytes,
+                         gdn2_stream_t stream);
+/* Backward; `workspace` as gdn2_linear_attn_fwd left it under GDN2_SAVE_FOR_BWD
+ * for the same arguments.  Every gradient is reduced in a fixed order. */
+size_t gdn2_linear_attn_bwd_workspace_size(const gdn2_linear_attn_args* a);
+int gdn2_linear_attn_bwd(const gdn2_linear_attn_args* a, const gdn2_linear_attn_grads* gr, const void* workspace,
+                         size_t workspace_bytes, void* bwd_workspace, size_t bwd_workspace_bytes,
+                         gdn2_stream_t stream);
+/* Token-serial form (decoding): each sequence's state is read once, taken
+ * through its tokens and written once (to ht, with GDN2_STORE_FINAL). */
+int gdn2_linear_attn_recurrent_fwd(const gdn2_linear_attn_args* a, gdn2_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* layer norm                                                                */
+/* ------------------------------------------------------------------------- */
+/*
+ * Per row of D (1 <= D <= 32768), with s = x, or s = x + residual:
+ *     y = (s - mean(s)) * rstd * weight + bias,  rstd = 1 / sqrt(var(s) + eps)
+ * x, y: `dtype`; residual and s: `dtype_residual` (s is rounded to it before
+ * the statistics, so y is a function of the s that is returned); weight, bias:
+ * `dtype_weight`, either may be NULL.  mean, rstd: fp32 [rows], kept for the
+ * backward.  Rows are contiguous.  The backward takes dy and, with a residual,
+ * ds (the cotangent of the returned s, or NULL) and writes dx (`dtype`),
+ * dresidual (`dtype_residual`), dweight and dbias (`dtype_weight`), the last
+ * two summed in fp32 in a fixed order.
+ */
+typedef struct gdn2_layer_norm_args {
+  int64_t rows, D;
+  float eps;
+  int32_t dtype, dtype_residual, dtype_weight;
+  const void* x;
+  const void* residual;   /* or NULL */
+  const void* weight;     /* or NULL */
+  const void* bias;       /* or NULL */
+  void* y;
+  void* s;                /* with residual */
+  float* mean;            /* or NULL with rstd (nothing kept) */
+  float* rstd;
+} gdn2_layer_norm_args;
+
+typedef struct gdn2_layer_norm_grads {
+  const void* dy;
+  const void* ds;         /* or NULL */
+  const void* s;          /* the rows that were normalised: s, or x without a residual */
+  void* dx;
+  void* dresidual;        /* with residual, or NULL */
+  void* dweight;          /* or NULL */
+  void* dbias;            /* or NULL */
+} gdn2_layer_norm_grads;
+
+int gdn2_layer_norm_fwd(const gdn2_layer_norm_args* a, gdn2_stream_t stream);
+size_t gdn2_layer_norm_bwd_workspace_size(const gdn2_layer_norm_args* a);
+/* reads a->weight, mean, rstd; a->residual != NULL says that s is in dtype_residual */
+int gdn2_layer_norm_bwd(const gdn2_layer_norm_args* a, const gdn2_layer_norm_grads* g, void* workspace,
+                        size_t workspace_bytes, gdn2_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
 /* opt-in per-kernel timing (measurement hook, no reference counterpart)     */
 /* ------------------------------------------------------------------------- */
 /* While enabled, every launch of the library is bracketed by CUDA events on
