@@ -2,11 +2,15 @@
 // the launchers behind the gdn2_linear_attn_* entry points.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace gdn2 {
 
-constexpr int kLaChunkF32 = 64;  // tokens per chunk of the fp32 kernels
+constexpr int kLaChunkF32 = 64;   // tokens per chunk of the fp32 kernels
+constexpr int kLaChunkTc = 128;   // and of the tensor-core kernels
+constexpr int kLaSms = 148;       // CTAs of a persistent kernel: one per SM of a B200
 
 // A chunk of a packed batch: its sequence (-1: past the last chunk) and its index there.
 struct LaChunk {
@@ -46,24 +50,85 @@ struct LaGeom {
   }
 };
 
+// Sequences cut into segments of `len` chunks for the scans over time, so that
+// few sequences and heads over a long axis still fill the GPU.
+struct LaSegs {
+  int len;              // chunks per segment
+  bool multi;           // some sequence may have several
+  int64_t per;          // segments per sequence (dense)
+  int64_t entries;      // segments over all sequences (packed and cut: an upper bound)
+  const LaChunk* map;   // [entries] (sequence, segment), packed and cut only
+  const int32_t* first; // [N + 1] first entry of each sequence
+  float* X;             // [entries, HV, K, V] states, where cut
+  float* D;             // [entries, HV] decay over the segment
+  GDN2_DEV bool get(int64_t entry, const LaGeom&, int64_t& n, int64_t& s) const {
+    if (map) {
+      n = map[entry].n;
+      s = map[entry].c;
+      return n >= 0;
+    }
+    n = entry / per;
+    s = entry - n * per;
+    return true;
+  }
+  GDN2_DEV int64_t first_of(int64_t n) const { return map ? (int64_t)first[n] : n * per; }
+};
+
+struct LaSegWs {
+  LaChunk* map;
+  int32_t* first;
+  float* X;
+  float* D;
+};
+
 struct LaWs {
   LaChunk* map;     // [NT]   packed only
   int32_t* first;   // [N+1]  packed only
   float* total;     // [NT, HV] exp of each chunk's summed decay (fp32 kernels)
   float* states;    // [NT, HV, K, V] fp32 (fp32 kernels)
+  __nv_bfloat16* states16;  // [NT, HV, K, V] bf16 (tensor-core kernels, for the backward)
+  LaSegWs seg;
 };
 struct LaBwdWs {
   float* dstates;   // [NT, HV, K, V] fp32 (fp32 kernels)
   float* dg;        // [B, T, HV] fp32, the terms of a per-head decay's gradient
 };
 
-inline int la_chunk(const gdn2_linear_attn_args&) { return kLaChunkF32; }
+// the simple path also runs bf16 training until its backward is on the tensor cores
+inline bool la_tc(const gdn2_linear_attn_args& a) {
+  return a.dtype == GDN2_BF16 && !(a.flags & GDN2_SAVE_FOR_BWD);
+}
+inline int la_chunk(const gdn2_linear_attn_args& a) { return la_tc(a) ? kLaChunkTc : kLaChunkF32; }
 
 // chunks over all sequences: exact for dense batches, an upper bound for packed
 // ones (the lengths stay on the device): sum ceil(len / C) <= T / C + N
 inline int64_t la_num_chunks(const gdn2_linear_attn_args& a) {
   const int64_t C = la_chunk(a);
   return a.cu_seqlens ? a.T / C + a.N : a.B * ((a.T + C - 1) / C);
+}
+
+// The cut of the scans: enough segments for one per SM and 64-column slice of a
+// head, none shorter than 8 chunks (a cut costs a second pass over k and v).
+inline LaSegs la_segs(const gdn2_linear_attn_args& a, const LaSegWs& ws) {
+  const int64_t C = kLaChunkTc, NT = la_num_chunks(a), slices = a.HV * (a.V / 64);
+  const int64_t most = a.cu_seqlens ? (a.T + C - 1) / C : (a.T + C - 1) / C;  // chunks of the longest sequence
+  const int64_t want = std::max<int64_t>(1, kLaSms / slices);                 // segments over all sequences
+  LaSegs g{};
+  int64_t len = most;
+  if (a.cu_seqlens) len = (NT + want - 1) / want;
+  else if (a.N < want) len = (most + want / std::max<int64_t>(a.N, 1) - 1) / (want / std::max<int64_t>(a.N, 1));
+  len = std::max<int64_t>(len, 8);
+  g.multi = len < most;
+  g.len = (int)(g.multi ? len : std::max<int64_t>(most, 1));
+  g.per = g.multi ? (most + len - 1) / len : 1;
+  g.entries = a.cu_seqlens ? (g.multi ? a.T / (C * len) + a.N : a.N) : a.N * g.per;
+  if (g.multi) {
+    g.map = a.cu_seqlens ? ws.map : nullptr;
+    g.first = ws.first;
+    g.X = ws.X;
+    g.D = ws.D;
+  }
+  return g;
 }
 
 inline size_t la_align(size_t x) { return (x + 255) & ~size_t(255); }
@@ -77,9 +142,24 @@ inline size_t la_ws_layout(const gdn2_linear_attn_args& a, void* base, LaWs* out
   };
   LaWs w{};
   const size_t NT = (size_t)la_num_chunks(a), HV = (size_t)a.HV, KV = (size_t)(a.K * a.V);
-  if (a.cu_seqlens) {
+  const bool save = a.flags & GDN2_SAVE_FOR_BWD;
+  if (a.cu_seqlens && (save || !la_tc(a))) {
     w.map = (LaChunk*)take(NT * sizeof(LaChunk));
     w.first = (int32_t*)take(((size_t)a.N + 1) * 4);
+  }
+  if (la_tc(a)) {
+    const LaSegs g = la_segs(a, w.seg);
+    if (g.multi) {
+      if (a.cu_seqlens) {
+        w.seg.map = (LaChunk*)take((size_t)g.entries * sizeof(LaChunk));
+        w.seg.first = (int32_t*)take(((size_t)a.N + 1) * 4);
+      }
+      w.seg.X = (float*)take((size_t)g.entries * HV * KV * 4);
+      w.seg.D = (float*)take((size_t)g.entries * HV * 4);
+    }
+    if (save) w.states16 = (__nv_bfloat16*)take(NT * HV * KV * 2);
+    if (out) *out = w;
+    return off;
   }
   w.total = (float*)take(NT * HV * 4);
   w.states = (float*)take(NT * HV * KV * 4);
@@ -107,9 +187,9 @@ inline LaGeom la_geom(const gdn2_linear_attn_args& a, const LaWs& ws) {
   return LaGeom{a.cu_seqlens, a.T, a.N, C, (a.T + C - 1) / C, ws.map, ws.first};
 }
 
-// The log-decay of one token.  Values below -1e5 (and -inf) count as -1e5:
-// exp of it is zero in fp32 and sums of it stay exact to 1e-10 in fp64, so
-// differences of running sums never become inf - inf.  NaN stays NaN.
+// The log-decay of one token.  Values below -150 (and -inf) count as -150: exp
+// of it is zero in fp32, and differences of running sums never become
+// inf - inf.  NaN stays NaN.
 struct LaDecay {
   const void* g;
   int64_t sb, st, sh;
@@ -119,7 +199,7 @@ struct LaDecay {
     const int64_t i = kind == GDN2_DECAY_HEAD ? hv * sh : b * sb + t * st + hv * sh;
     const float x = dtype == GDN2_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i])
                                        : static_cast<const float*>(g)[i];
-    return x < -1e5f ? -1e5 : (double)x;
+    return x < -150.f ? -150.0 : (double)x;
   }
 };
 inline LaDecay la_decay(const gdn2_linear_attn_args& a) {
@@ -129,6 +209,9 @@ inline LaDecay la_decay(const gdn2_linear_attn_args& a) {
 int la_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s);
 int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
                          const LaBwdWs& bw, cudaStream_t s);
+int la_tc_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s);
+// fault word of the tensor-core kernels: bit 0 = a bounded wait gave up
+int la_fault_read(int clear, unsigned int* out);
 int la_recurrent_launch(const gdn2_linear_attn_args& a, cudaStream_t s);
 
 int layer_norm_fwd_launch(const gdn2_layer_norm_args& a, cudaStream_t s);

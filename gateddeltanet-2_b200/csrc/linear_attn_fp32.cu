@@ -475,8 +475,9 @@ __global__ void __launch_bounds__(256) la_head_sum_kernel(const float* dg, int64
 }
 
 // (sequence, chunk) of every chunk id of a packed batch, and each sequence's
-// first chunk: one CTA walks the lengths 1024 at a time with a block prefix sum.
-__global__ void __launch_bounds__(1024) la_chunk_map_kernel(LaGeom geo, LaChunk* map, int32_t* first, int64_t NT) {
+// first chunk; the same for segments, of which an empty sequence has one.  One CTA walks the lengths 1024 at a time with a block prefix sum.
+__global__ void __launch_bounds__(1024) la_chunk_map_kernel(LaGeom geo, int64_t unit, int64_t least, LaChunk* map,
+                                                            int32_t* first, int64_t NT) {
   __shared__ int64_t warp_sum[32];
   __shared__ int64_t carry;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(1024) la_chunk_map_kernel(LaGeom geo, LaChunk*
     const int64_t n = n0 + tid;
     int64_t bos = 0, len = 0;
     if (n < geo.N) geo.seq(n, bos, len);
-    const int64_t nch = (len + geo.C - 1) / geo.C;
+    const int64_t nch = n < geo.N ? max((len + unit - 1) / unit, least) : 0;
     int64_t s = nch;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -638,19 +639,46 @@ struct BwdCall {
 }  // namespace
 
 int la_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
+  const LaGeom geo = la_geom(a, ws);
+  const bool any = a.B * a.T > 0;
   if (a.cu_seqlens) {
-    la_chunk_map_kernel<<<1, 1024, 0, s>>>(la_geom(a, ws), ws.map, ws.first, la_num_chunks(a));
-    GDN2_LAUNCH_CHECK();
-    const int64_t e = a.dtype == GDN2_BF16 ? 2 : 4;
-    la_zero_outside_kernel<<<32, 256, 0, s>>>(LaRows{{a.o}, {a.HV * a.V * e}}, la_geom(a, ws));
-    GDN2_LAUNCH_CHECK();
+    if (ws.map) {
+      la_chunk_map_kernel<<<1, 1024, 0, s>>>(geo, geo.C, 0, ws.map, ws.first, la_num_chunks(a));
+      GDN2_LAUNCH_CHECK();
+    }
+    if (ws.seg.map) {
+      const LaSegs seg = la_segs(a, ws.seg);
+      la_chunk_map_kernel<<<1, 1024, 0, s>>>(geo, (int64_t)geo.C * seg.len, 1, ws.seg.map, ws.seg.first, seg.entries);
+      GDN2_LAUNCH_CHECK();
+    }
+    if (any) {
+      const int64_t e = a.dtype == GDN2_BF16 ? 2 : 4;
+      la_zero_outside_kernel<<<32, 256, 0, s>>>(LaRows{{a.o}, {a.HV * a.V * e}}, geo);
+      GDN2_LAUNCH_CHECK();
+    }
   }
+  if (!any) {  // no tokens: the final states are the initial ones
+    if (!(a.flags & GDN2_STORE_FINAL)) return 0;
+    const size_t bytes = (size_t)(a.N * a.HV * a.K * a.V) * 4;
+    if (a.flags & GDN2_HAS_H0) GDN2_CUDA_TRY(cudaMemcpyAsync(a.ht, a.h0, bytes, cudaMemcpyDeviceToDevice, s));
+    else GDN2_CUDA_TRY(cudaMemsetAsync(a.ht, 0, bytes, s));
+    return 0;
+  }
+  if (la_tc(a)) return la_tc_fwd_launch(a, ws, s);
   const FwdCall f{a, ws, s};
   return a.dtype == GDN2_F32 ? by_dims<float>(a, f) : by_dims<__nv_bfloat16>(a, f);
 }
 
 int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
                   const LaBwdWs& bw, cudaStream_t s) {
+  if (a.B * a.T == 0) {
+    const size_t bytes = (size_t)(a.N * a.HV * a.K * a.V) * 4;
+    if (gr.dh0 && gr.dht) GDN2_CUDA_TRY(cudaMemcpyAsync(gr.dh0, gr.dht, bytes, cudaMemcpyDeviceToDevice, s));
+    else if (gr.dh0) GDN2_CUDA_TRY(cudaMemsetAsync(gr.dh0, 0, bytes, s));
+    if (gr.dg && a.decay == GDN2_DECAY_HEAD)
+      GDN2_CUDA_TRY(cudaMemsetAsync(gr.dg, 0, (size_t)a.HV * (a.dtype_g == GDN2_BF16 ? 2 : 4), s));
+    return 0;
+  }
   if (a.cu_seqlens) {
     const int64_t e = a.dtype == GDN2_BF16 ? 2 : 4, eg = a.dtype_g == GDN2_BF16 ? 2 : 4;
     const bool token = a.decay == GDN2_DECAY_TOKEN;

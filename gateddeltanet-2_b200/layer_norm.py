@@ -19,7 +19,7 @@ class LayerNormFunction(torch.autograd.Function):
     """``(y, s)`` of ``s = x + residual``, ``y = LN(s)``; ``y`` alone without a residual."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, residual):
+    def forward(ctx, x, weight, bias, eps, residual, grad):
         D = x.shape[-1]
         xs = x.contiguous()
         rows = xs.numel() // D
@@ -28,7 +28,7 @@ class LayerNormFunction(torch.autograd.Function):
         b = None if bias is None else bias.contiguous()
         y = torch.empty_like(xs)
         s = None if rs is None else torch.empty_like(rs)
-        save = any(ctx.needs_input_grad)
+        save = grad and any(ctx.needs_input_grad)  # needs_input_grad alone is also set under no_grad
         stats = torch.empty(2, rows, device=x.device, dtype=torch.float32) if save else None
         ptr = _lib.ptr
         wt = w if w is not None else b
@@ -70,7 +70,7 @@ class LayerNormFunction(torch.autograd.Function):
             grads = _lib.LayerNormGrads(dy.data_ptr(), ptr(ds), s.data_ptr(), ptr(dx), ptr(dr), ptr(dw), ptr(db))
             _lib.check(lib.gdn2_layer_norm_bwd(args, grads, ws.data_ptr(), size, _lib.stream_ptr(dev)),
                        "gdn2_layer_norm_bwd")
-        return (dr if shared else dx) if need[0] else None, dw, db, None, dr
+        return (dr if shared else dx) if need[0] else None, dw, db, None, dr, None
 
 
 @torch.compiler.disable
@@ -111,7 +111,7 @@ def layer_norm(
         if t is not None and t.device != x.device:
             raise ValueError(f"{name} is on {t.device}, x on {x.device}.")
     _lib.require_device(x)
-    return LayerNormFunction.apply(x, weight, bias, float(eps), residual)
+    return LayerNormFunction.apply(x, weight, bias, float(eps), residual, torch.is_grad_enabled())
 
 
 class LayerNorm(nn.Module):

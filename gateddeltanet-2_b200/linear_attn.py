@@ -110,14 +110,14 @@ class ChunkLinearAttnFunction(torch.autograd.Function):
     """Autograd wrapper over ``gdn2_linear_attn_fwd`` / ``gdn2_linear_attn_bwd``."""
 
     @staticmethod
-    def forward(ctx, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, N):
+    def forward(ctx, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, N, grad):
         B, T, H, K = q.shape
         HV, V = v.shape[2:]
         q, k, v = _strided(q), _strided(k), _strided(v)
         h0 = None if initial_state is None else initial_state.contiguous()
         o = torch.empty(B, T, HV, V, device=q.device, dtype=q.dtype)
         ht = torch.empty(N, HV, K, V, device=q.device, dtype=torch.float32) if output_final_state else None
-        save = any(ctx.needs_input_grad)
+        save = grad and any(ctx.needs_input_grad)  # needs_input_grad alone is also set under no_grad
         lib = _lib.load()
         with _lib.on_device(q.device):
             args = _args(q, k, v, g, h0, ht, o, scale, N, cu_seqlens, _lib.SAVE_FOR_BWD if save else 0)
@@ -149,7 +149,7 @@ class ChunkLinearAttnFunction(torch.autograd.Function):
             grads = _lib.LinearAttnGrads(ptr(do), ptr(dht), ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(dh0))
             _lib.check(lib.gdn2_linear_attn_bwd(args, grads, ws.data_ptr(), ws.numel(), bws.data_ptr(), size,
                                                 _lib.stream_ptr(q.device)), "gdn2_linear_attn_bwd")
-        return dq, dk, dv, dg, None, dh0, None, None, None
+        return dq, dk, dv, dg, None, dh0, None, None, None, None
 
 
 @torch.compiler.disable
@@ -188,7 +188,7 @@ def chunk_linear_attn(
     if scale is None:
         scale = q.shape[-1] ** -0.5
     return ChunkLinearAttnFunction.apply(q, k, v, g, float(scale), initial_state, output_final_state,
-                                         _cu(cu_seqlens), N)
+                                         _cu(cu_seqlens), N, torch.is_grad_enabled())
 
 
 @torch.compiler.disable

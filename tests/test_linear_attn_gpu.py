@@ -89,6 +89,15 @@ def run_both(gdn2, d, lens=None, scale=None, final=True, use_dht=True):
         outs, cots = outs + [ht], cots + [d["dht"].cuda()]
     grads = torch.autograd.grad(outs, list(own.values()), cots)
     got = dict(o=o, ht=ht, **{"d" + n: x for n, x in zip(names, grads)})
+    with torch.no_grad():  # nothing kept for a backward: the prompt's form, with and without the final state
+        got["o_p"], got["ht_p"] = gdn2.chunk_linear_attn(own["q"], own["k"], own["v"], own.get("g"), scale=scale,
+                                                         initial_state=own.get("h0"), output_final_state=True,
+                                                         cu_seqlens=cu)
+        got["o_n"], none = gdn2.chunk_linear_attn(own["q"], own["k"], own["v"], own.get("g"), scale=scale,
+                                                  initial_state=own.get("h0"), cu_seqlens=cu)
+        assert none is None
+    want.update(o_p=want["o"], ht_p=want["ht"], o_n=want["o"])
+    assert gdn2._lib.device_fault_read() == 0
     return got, want
 
 
@@ -98,11 +107,11 @@ def dg_mass(d, want):
     return float(m)
 
 
-def check(got, want, d, dtype, names=("o", "ht", "dq", "dk", "dv", "dg", "dh0")):
+def check(got, want, d, dtype, names=("o", "ht", "dq", "dk", "dv", "dg", "dh0", "o_p", "ht_p", "o_n")):
     for n in names:
         if n not in got or got[n] is None:
             continue
-        tol = STATE_TOL if n in ("ht", "dh0") else TOL[dtype]
+        tol = STATE_TOL if n in ("ht", "ht_p", "dh0") else TOL[dtype]
         if n == "dg":
             err = (got[n].detach().double().cpu() - want[n]).norm() / want[n].numel() ** 0.5
             ref = want[n].norm() / want[n].numel() ** 0.5
