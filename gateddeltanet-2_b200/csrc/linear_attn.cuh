@@ -194,13 +194,17 @@ struct LaDecay {
   const void* g;
   int64_t sb, st, sh;
   int kind, dtype;
-  GDN2_DEV double at(int64_t b, int64_t t, int64_t hv) const {
-    if (kind == GDN2_DECAY_NONE) return 0.0;
+  // the bits as they lie in memory (to be loaded ahead), and their value
+  GDN2_DEV uint32_t raw(int64_t b, int64_t t, int64_t hv) const {
+    if (kind == GDN2_DECAY_NONE) return 0;
     const int64_t i = kind == GDN2_DECAY_HEAD ? hv * sh : b * sb + t * st + hv * sh;
-    const float x = dtype == GDN2_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(g)[i])
-                                       : static_cast<const float*>(g)[i];
+    return dtype == GDN2_BF16 ? static_cast<const uint16_t*>(g)[i] : static_cast<const uint32_t*>(g)[i];
+  }
+  GDN2_DEV double value(uint32_t bits) const {
+    const float x = __uint_as_float(dtype == GDN2_BF16 ? bits << 16 : bits);
     return x < -150.f ? -150.0 : (double)x;
   }
+  GDN2_DEV double at(int64_t b, int64_t t, int64_t hv) const { return value(raw(b, t, hv)); }
 };
 inline LaDecay la_decay(const gdn2_linear_attn_args& a) {
   return LaDecay{a.g, a.g_stride[0], a.g_stride[1], a.g_stride[2], a.decay, a.dtype_g};

@@ -10,21 +10,23 @@
 // CTAs side by side share q and k through L2.  CTAs are persistent: the roles
 // below run through the chunks of all its tasks as one pipeline, so a task's
 // loads overlap the end of the one before.
-//   warp 0      TMA loads into two stages (q, k; v)
-//   warp 1      allocates TMEM, issues the MMAs: Q K^T (the next chunk's), Q S,
-//               K^T (w v), P V (P from TMEM)
-//   warp 2      running sums of g in fp64 and the factors made from them
-//   warp 3      TMA stores: o, the chunk's entering state
-//   warps 4-7   scores: Q K^T out of TMEM, decayed, back as the bf16 operand P.
-//               Off the diagonal e^{G_i - G_j} = e^{G_i - G_r} e^{G_r - G_j} with r
-//               the first row of the 32-row block: both factors are at most 1 for
-//               decays, one is per row, the other per block and column, so only the
-//               32 diagonal columns take an exponential each.
-//   warps 8-11  w v in bf16, and the state in registers (thread = row k of S):
+//   warp 0      TMA loads (q, k: two stages, three without outputs; v: three)
+//   warp 1      allocates TMEM, issues the MMAs
+//   warp 2      running sums of g in fp64, handed on as pairs of floats
+//   warp 3      TMA stores of the chunks' entering states
+//   warps 4-11  scores (64 columns per four warps): Q K^T out of TMEM, decayed,
+//               back as the bf16 operand P.  Off the diagonal e^{G_i - G_j} =
+//               e^{G_i - G_r} e^{G_r - G_j} with r the first row of the 32-row block:
+//               both factors are at most 1 for decays, one is per row, the other per
+//               block and column, so only the 32 diagonal columns take an exponential each.
+//   warps 12-15 w v in bf16, and the state in registers (thread = row k of S):
 //               S <- e^{G_C} S + what the MMA left in TMEM; bf16 copy for Q S
-//   warps 12-15 o out of TMEM (thread = token), bf16, into the stage's own v slot
-// Precision: P, S and w v are rounded to bf16 as MMA operands (2^-9 each, as the
-// result itself).  Where the final state (or the initial state's gradient) is
+//   warps 16-19 o out of TMEM (thread = token), straight to memory, 32 bytes a store
+// MMA order per chunk i: Q K^T, K^T (w v), then P V of chunk i - 1, then Q S.  The
+// lag gives the scores more than a chunk's time, and a q, k stage is held only
+// from its first product to its last, so two stages cover the loads' latency.
+// Precision: P, S, w and w v are rounded to bf16 for the MMAs (as the result
+// itself is).  Where the final state (or the initial state's gradient) is
 // asked for, w v goes in as the sum of two bf16 values, so the state that leaves
 // in fp32 carries 16 bits or more of every product.
 // Every wait is bounded (tc::kWaitLimitNs); one that gives up sets g_la_fault.
@@ -47,30 +49,33 @@ constexpr int kC = kLaChunkTc;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kTile = 128 * 64 * 2;  // one [128 x 64] bf16 swizzled tile
 
-struct alignas(16) Factors {  // of one chunk; cf[w - 1][j] = e^{G_{32 w} - G_j}, j < 32 w
-  float rowE[kC];     // e^{G_i}
-  float r[kC];        // e^{G_i - G_{32 floor(i / 32)}}
-  float g2[kC];       // (G_i - G_{32 floor(i / 32)}) log2 e
-  float yw[kC];       // e^{G_C - G_j} (backwards: scale e^{G_i}); 0 past the last token
-  float cf[3][kC];
-  float total;        // e^{G_C}
+// Running sums of one chunk's log-decays: fp64 values as a float and what it
+// misses (8 bits of that are plenty)
+struct alignas(16) Sums {
+  float hi[kC];
+  __nv_bfloat16 lo[kC];
 };
+// e^x: the hardware's base-2 exponential (2^-22) of x log2 e (rounded: another 2^-24 |x|)
+GDN2_DEV float exp_of(float x) { return exp2_approx(x * kLog2e); }
+// G_i - G_j
+GDN2_DEV float sum_diff(const Sums& g, int i, int j) {
+  return (g.hi[i] - g.hi[j]) + (__bfloat162float(g.lo[i]) - __bfloat162float(g.lo[j]));
+}
 
-template <int K, bool kOut>
+template <int K, bool kOut, bool kExact>
 struct alignas(1024) ScanSmem {
-  __nv_bfloat16 X[2][K / 64][128 * 64];
-  __nv_bfloat16 Q[kOut ? 2 : 1][kOut ? K / 64 : 1][kOut ? 128 * 64 : 512];
-  __nv_bfloat16 Y[2][128 * 64];
-  __nv_bfloat16 YW[2][128 * 64];  // two chunks' w v, or (exact) the two terms of one
-  __nv_bfloat16 S[K * 64];        // bf16 state, rows k
-  Factors f[2];
-  uint64_t full_x[2], full_y[2], empty_x[2], empty_y[2], f_full[2], f_empty[2], qk_full[2], p_full[2], ds_full[2];
-  uint64_t yw_full[2], o_staged[2], s_full, s_free, o_full, o_free;
+  static constexpr int NX = kOut ? 2 : 3, NY = 3;  // stages
+  static constexpr int NB = kOut ? 1 : 2;          // chunks of w v held
+  __nv_bfloat16 X[NX][(kOut ? 2 : 1) * K / 64][128 * 64];  // k; with outputs then q
+  __nv_bfloat16 Y[NY][128 * 64];
+  __nv_bfloat16 YW[NB][kExact ? 2 : 1][128 * 64];
+  __nv_bfloat16 S[K * 64];  // bf16 state, rows k
+  Sums f[2];
+  float cw[kOut ? 320 : 4];  // column factors of the score warps, 32 (w + 1) for w = 0..3
+  uint64_t full_x[NX], empty_x[NX], full_y[NY], empty_y[NY], f_full[2], f_empty[2], qk_full[2], p_full[2];
+  uint64_t yw_full[NB], ds_full[NB], s_full, s_free, o_full, o_free, aborted;
   uint32_t tbase;
 };
-
-static_assert(sizeof(Factors) % 16 == 0 && offsetof(Factors, g2) % 16 == 0 && offsetof(Factors, cf) % 16 == 0,
-              "16-byte reads of the factors");
 
 struct ScanArgs {
   gdn2_linear_attn_args a;
@@ -90,13 +95,12 @@ struct Task {
 };
 
 template <bool kBack>
-GDN2_DEV bool get_task(const ScanArgs& p, int64_t id, Task& t) {
-  const int vs = (int)(p.a.V >> 6);
-  t.z = (int)(id % vs);
-  const int64_t r = id / vs;
-  t.hv = r % p.a.HV;
-  t.entry = r / p.a.HV;
-  t.h = t.hv / (p.a.HV / p.a.H);
+GDN2_DEV bool find_task(const ScanArgs& p, int64_t id, Task& t) {
+  const uint32_t vs = (uint32_t)(p.a.V >> 6), HV = (uint32_t)p.a.HV, r = (uint32_t)id / vs;
+  t.z = (int)((uint32_t)id % vs);
+  t.hv = r % HV;
+  t.entry = r / HV;
+  t.h = (uint32_t)t.hv / (HV / (uint32_t)p.a.H);
   int64_t s;
   if (!p.seg.get(t.entry, p.geo, t.n, s)) return false;
   p.geo.seq(t.n, t.bos, t.len);
@@ -111,47 +115,101 @@ GDN2_DEV bool get_task(const ScanArgs& p, int64_t id, Task& t) {
   return true;
 }
 
-GDN2_DEV uint64_t kmaj(const void* p, int kk) {  // K-major tile, 16-column step kk
-  return tc::sdesc_sw128(tc::smem_u32(p) + kk * 32, 16, 1024);
+// A value that all lanes share, in a form that the compiler knows to be shared:
+// loops and branches on it are then known to keep the warp converged, and the
+// shuffles inside them are single instructions instead of ten.
+template <typename T>
+GDN2_DEV T uniform(T x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// find_task for a whole warp
+template <bool kBack>
+GDN2_DEV bool get_task(const ScanArgs& p, int64_t id, Task& t) {
+  const bool any = __all_sync(0xffffffffu, find_task<kBack>(p, id, t));
+  t.n = uniform(t.n);
+  t.bos = uniform(t.bos);
+  t.len = uniform(t.len);
+  t.cb = uniform(t.cb);
+  t.ce = uniform(t.ce);
+  t.head = __all_sync(0xffffffffu, t.head);
+  t.tail = __all_sync(0xffffffffu, t.tail);
+  return any;
 }
-GDN2_DEV uint64_t nmaj(const void* p, int kk) {  // M- or N-major tile, 16-row step kk; 64-column blocks one tile apart
-  return tc::sdesc_sw128(tc::smem_u32(p) + kk * 2048, kTile, 1024);
+
+// Operand descriptors from a shared-memory address in 16-byte units: the low
+// word is that address plus constants, the high word a constant (8-row groups
+// 1024 bytes apart, version 1, 128-byte swizzle).
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+GDN2_DEV uint64_t desc(uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | lo; }
+GDN2_DEV uint32_t addr16(const void* p) { return tc::smem_u32(p) >> 4; }
+// K-major tiles of 64 columns, 16-column step kk over all of them
+GDN2_DEV uint64_t kmaj(uint32_t a16, int kk) { return desc(a16 + (kk >> 2) * (kTile >> 4) + (kk & 3) * 2 + (1u << 16)); }
+// M- or N-major tile, 16-row step kk; 64-column blocks one tile apart
+GDN2_DEV uint64_t nmaj(uint32_t a16, int kk) { return desc(a16 + kk * 128 + ((kTile >> 4) << 16)); }
+// a whole 32-byte sector per thread where the tensor allows it
+GDN2_DEV void st_32bytes(void* p, const uint4& a, const uint4& b) {
+  if ((reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+                 "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+  } else {
+    static_cast<uint4*>(p)[0] = a;
+    static_cast<uint4*>(p)[1] = b;
+  }
+}
+// Bounded waits.  One lane: the retry loop is one copy of code.  A whole warp:
+// votes keep it converged in a way that the compiler can see (a call would not).
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity) { return tc::mbar_wait(bar, parity); }
+GDN2_DEV bool wait(uint64_t* bar, uint32_t parity) {
+  return tc::mbar_try_wait(tc::smem_u32(bar), parity) || wait_slow(bar, parity);
 }
 GDN2_DEV bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity));
+  const uint32_t addr = tc::smem_u32(bar);
+  bool r = __all_sync(0xffffffffu, tc::mbar_try_wait(addr, parity));
+  if (!r) {
+    const uint64_t t0 = tc::globaltimer_ns();
+    do {
+      r = __all_sync(0xffffffffu, tc::mbar_try_wait(addr, parity));
+    } while (!r && __all_sync(0xffffffffu, tc::globaltimer_ns() - t0 < tc::kWaitLimitNs));
+  }
+  return r;
 }
 
 template <int K, bool kOut, bool kStore, bool kBack, bool kExact>
-__global__ void __launch_bounds__(kOut ? 512 : 256, 1)
-la_scan_kernel(const ScanArgs p, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmQ,
-               const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmO,
-               const __grid_constant__ CUtensorMap tmS) {
-  extern __shared__ unsigned char smem_raw[];
-  using Sm = ScanSmem<K, kOut>;
-  Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr bool kS16 = kOut || kStore;  // the bf16 state is used
-  constexpr uint32_t kColQK = 0, kColO1 = 256, kColO2 = 320, kColDS = kOut ? 384 : 0;
+__global__ void __launch_bounds__(kOut ? 640 : 256, 1)
+la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmQ,
+               const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmS) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  using Sm = ScanSmem<K, kOut, kExact>;
+  Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
+  constexpr uint32_t NX = Sm::NX, NY = Sm::NY, NB = Sm::NB;
+  // TMEM columns: two score buffers, Q S of two chunks, P V, the state term
+  constexpr uint32_t kColQK = 0, kColO1 = 256, kColO2 = 384, kColDS = kOut ? 448 : 0;
   constexpr uint32_t kCols = kOut ? 512 : 128;
-  constexpr int kNB = kExact ? 1 : 2;  // chunks of w v held
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (uint32_t i = 0; i < NX; ++i) {
       tc::mbar_init(&sm.full_x[i], 1);
-      tc::mbar_init(&sm.full_y[i], 1);
       tc::mbar_init(&sm.empty_x[i], 1);
-      tc::mbar_init(&sm.empty_y[i], kOut ? 1 : 128);
-      tc::mbar_init(&sm.f_full[i], 32);
-      tc::mbar_init(&sm.f_empty[i], kOut ? 12 : 4);
-      tc::mbar_init(&sm.qk_full[i], 1);
-      tc::mbar_init(&sm.p_full[i], 128);
-      tc::mbar_init(&sm.ds_full[i], 1);
-      tc::mbar_init(&sm.yw_full[i], 128);
-      tc::mbar_init(&sm.o_staged[i], 128);
     }
-      tc::mbar_init(&sm.s_full, 128);
+    for (uint32_t i = 0; i < NY; ++i) {
+      tc::mbar_init(&sm.full_y[i], 1);
+      tc::mbar_init(&sm.empty_y[i], kOut ? 1 : 128);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&sm.f_full[i], 32);
+      tc::mbar_init(&sm.f_empty[i], kOut ? 16 : 4);
+      tc::mbar_init(&sm.qk_full[i], 1);
+      tc::mbar_init(&sm.p_full[i], 256);
+    }
+    for (uint32_t i = 0; i < NB; ++i) {
+      tc::mbar_init(&sm.yw_full[i], 128);
+      tc::mbar_init(&sm.ds_full[i], 1);
+    }
+    tc::mbar_init(&sm.s_full, 128);
     tc::mbar_init(&sm.s_free, 1);
     tc::mbar_init(&sm.o_full, 1);
     tc::mbar_init(&sm.o_free, 128);
+    tc::mbar_init(&sm.aborted, 1);
     tc::mbar_fence_init();
   }
   if (warp == 1) tc::tmem_alloc(&sm.tbase, kCols);
@@ -175,111 +233,122 @@ la_scan_kernel(const ScanArgs p, const __grid_constant__ CUtensorMap tmX, const 
       tc::prefetch_tensormap(&tmY);
       if (kOut) tc::prefetch_tensormap(&tmQ);
       for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
-        if (!get_task<kBack>(p, id, t)) continue;
+        if (!find_task<kBack>(p, id, t)) continue;
         const int b = p.geo.cu ? 0 : (int)t.n;
         for (int i = 0; i < t.ce - t.cb; ++i, ++it) {
-          const int s = it & 1, tt = tok(nth(i));
-          const uint32_t par = ((it >> 1) & 1) ^ 1;
-          if (it >= 2 && !(ok = tc::mbar_wait(&sm.empty_x[s], par))) break;
-          tc::mbar_arrive_expect_tx(&sm.full_x[s], (kOut ? 2 : 1) * (K / 64) * kTile);
+          const uint32_t sx = it % NX, sy = it % NY;
+          const int tt = tok(nth(i));
+          if (it >= NY && !(ok = wait(&sm.empty_y[sy], (it / NY - 1) & 1))) break;
+          tc::mbar_arrive_expect_tx(&sm.full_y[sy], kTile);
+          tc::tma_load_4d(sm.Y[sy], &tmY, &sm.full_y[sy], 64 * t.z, (int)t.hv, tt, b);
+          if (it >= NX && !(ok = wait(&sm.empty_x[sx], (it / NX - 1) & 1))) {
+            wait(&sm.full_y[sy], (it / NY) & 1);
+            break;
+          }
+          tc::mbar_arrive_expect_tx(&sm.full_x[sx], (kOut ? 2 : 1) * (K / 64) * kTile);
 #pragma unroll
           for (int c = 0; c < K / 64; ++c) {
-            tc::tma_load_4d(sm.X[s][c], &tmX, &sm.full_x[s], 64 * c, (int)t.h, tt, b);
-            if constexpr (kOut) tc::tma_load_4d(sm.Q[s][c], &tmQ, &sm.full_x[s], 64 * c, (int)t.h, tt, b);
+            tc::tma_load_4d(sm.X[sx][c], &tmX, &sm.full_x[sx], 64 * c, (int)t.h, tt, b);
+            if constexpr (kOut) tc::tma_load_4d(sm.X[sx][K / 64 + c], &tmQ, &sm.full_x[sx], 64 * c, (int)t.h, tt, b);
           }
-          if (it >= 2 && !(ok = tc::mbar_wait(&sm.empty_y[s], par))) break;
-          tc::mbar_arrive_expect_tx(&sm.full_y[s], kTile);
-          tc::tma_load_4d(sm.Y[s], &tmY, &sm.full_y[s], 64 * t.z, (int)t.hv, tt, b);
         }
       }
       // loads in flight land before the CTA exits, also after a wait that gave up
-      for (uint32_t j = it > 2 ? it - 2 : 0; !ok && j < it; ++j) {
-        tc::mbar_wait(&sm.full_x[j & 1], (j >> 1) & 1);
-        tc::mbar_wait(&sm.full_y[j & 1], (j >> 1) & 1);
+      for (uint32_t j = it > NY ? it - NY : 0; !ok && j < it; ++j) {
+        wait(&sm.full_x[j % NX], (j / NX) & 1);
+        wait(&sm.full_y[j % NY], (j / NY) & 1);
       }
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMAs
-    if (lane == 0) {
+    if (tc::elect_one()) {
       constexpr uint32_t iQK = tc::idesc_bf16(128, 128, 0, 0), iNV = tc::idesc_bf16(128, 64, 0, 1);
       constexpr uint32_t iDS = tc::idesc_bf16(K, 64, 1, 1);
-      auto qk = [&](uint32_t j) {
-        const int s = j & 1;
-        if (!tc::mbar_wait(&sm.full_x[s], (j >> 1) & 1)) return false;
-        tc::tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < K / 16; ++kk)
-          tc::mma_bf16(tb + kColQK + 128 * s, kmaj(sm.Q[s][kk >> 2], kk & 3), kmaj(sm.X[s][kk >> 2], kk & 3), iQK,
-                       kk > 0);
-        tc::mma_commit(&sm.qk_full[s]);
-        return true;
-      };
+      const uint32_t aX = addr16(sm.X), aY = addr16(sm.Y), aW = addr16(sm.YW), aS = addr16(sm.S);
       uint32_t total = 0;  // chunks over all tasks
       for (int64_t id = blockIdx.x; id < p.tasks; id += step)
-        if (get_task<kBack>(p, id, t)) total += (uint32_t)max(t.ce - t.cb, 0);
-      if (kOut && total > 0) ok = qk(0);
-      for (; ok && it < total; ++it) {
-        const int s = it & 1, y = kNB == 2 ? s : 0;
-        if constexpr (kOut) {
-          if (!(ok = tc::mbar_wait(&sm.s_full, it & 1))) break;
-          if (it > 0 && !(ok = tc::mbar_wait(&sm.o_free, (it - 1) & 1))) break;
+        if (find_task<kBack>(p, id, t)) total += (uint32_t)max(t.ce - t.cb, 0);
+      for (; it < total + (kOut && total > 0 ? 1 : 0); ++it) {
+        const uint32_t s = it & 1, sx = it % NX, b = it % NB;
+        const uint32_t ax = aX + sx * (uint32_t)(sizeof(sm.X[0]) >> 4), aq = ax + (K / 64) * (kTile >> 4);
+        if (it < total) {
+          if (!(ok = wait(&sm.full_x[sx], (it / NX) & 1))) break;
+          if constexpr (kOut) {
+            tc::tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < K / 16; ++kk)
+              tc::mma_bf16(tb + kColQK + 128 * s, kmaj(aq, kk), kmaj(ax, kk), iQK,
+                           kk > 0);
+            tc::mma_commit(&sm.qk_full[s]);
+          }
+          if (!(ok = wait(&sm.yw_full[b], (it / NB) & 1))) break;
           tc::tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < K / 16; ++kk)
-            tc::mma_bf16(tb + kColO1, kmaj(sm.Q[s][kk >> 2], kk & 3), nmaj(sm.S, kk), iNV, kk > 0);
-        } else if (!(ok = tc::mbar_wait(&sm.full_x[s], (it >> 1) & 1))) {
-          break;
-        }
-        if (!(ok = tc::mbar_wait(&sm.yw_full[s], (it >> 1) & 1))) break;
-        tc::tc_fence_after();
+          for (int e = 0; e < (kExact ? 2 : 1); ++e)
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          tc::mma_bf16(tb + kColDS + 64 * s, nmaj(sm.X[s], kk), nmaj(sm.YW[y], kk), iDS, kk > 0);
-        if constexpr (kExact) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            tc::mma_bf16(tb + kColDS + 64 * s, nmaj(sm.X[s], kk), nmaj(sm.YW[1], kk), iDS, 1);
+            for (int kk = 0; kk < 8; ++kk)
+              tc::mma_bf16(tb + kColDS + 64 * b, nmaj(ax, kk),
+                                nmaj(aW + (b * (kExact ? 2 : 1) + e) * (kTile >> 4), kk), iDS, e + kk > 0);
+          tc::mma_commit(&sm.ds_full[b]);
+          if constexpr (!kOut) tc::mma_commit(&sm.empty_x[sx]);
         }
-        tc::mma_commit(&sm.ds_full[s]);
-        tc::mma_commit(&sm.empty_x[s]);
         if constexpr (kOut) {
-          if (it + 1 < total && !(ok = qk(it + 1))) break;
-          if (!(ok = tc::mbar_wait(&sm.full_y[s], (it >> 1) & 1) && tc::mbar_wait(&sm.p_full[s], (it >> 1) & 1))) break;
-          tc::tc_fence_after();
+          // chunk it - 2's outputs have left TMEM
+          if (it >= 2 && !(ok = wait(&sm.o_free, it & 1))) break;
+          if (it > 0) {
+            const uint32_t j = it - 1, sj = j & 1, sy = j % NY;
+            if (!(ok = wait(&sm.full_y[sy], (j / NY) & 1) && wait(&sm.p_full[sj], (j >> 1) & 1))) break;
+            tc::tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            tc::mma_bf16_ts(tb + kColO2, tb + kColQK + 128 * s + 8 * kk, nmaj(sm.Y[s], kk), iNV, kk > 0);
-          tc::mma_commit(&sm.o_full);
+            for (int kk = 0; kk < 8; ++kk)  // P: columns 0-31 and 64-95 of the score buffer
+              tc::mma_bf16_ts(tb + kColO2, tb + kColQK + 128 * sj + 8 * kk + (kk < 4 ? 0 : 32), nmaj(aY + sy * (kTile >> 4), kk), iNV,
+                              kk > 0);
+            tc::mma_commit(&sm.o_full);
+            tc::mma_commit(&sm.empty_y[sy]);
+          }
+          if (it < total) {
+            if (!(ok = wait(&sm.s_full, it & 1))) break;
+            tc::tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < K / 16; ++kk)
+              tc::mma_bf16(tb + kColO1 + 64 * s, kmaj(aq, kk), nmaj(aS, kk), iNV, kk > 0);
+            tc::mma_commit(&sm.empty_x[sx]);  // also: S has been read
+          }
         }
       }
-      // what was issued has completed before TMEM is released (the last commits, when all went well)
-      if (ok && total > 0) {
-        const uint32_t j = total - 1;
-        if (!(kOut ? tc::mbar_wait(&sm.o_full, j & 1) : tc::mbar_wait(&sm.ds_full[j & 1], (j >> 1) & 1))) ok = false;
-      } else if (!ok) {  // a commit of its own covers them
-        tc::mma_commit(&sm.o_full);
-        tc::mbar_wait(&sm.o_full, it & 1);
-      }
+      // what was issued has completed before TMEM is released
+      tc::mma_commit(&sm.aborted);
+      if (!wait(&sm.aborted, 0)) ok = false;
     }
   } else if (warp == 2) {
-    // -------------------------------------------------------------- factors
+    // ---------------------------------------------------------------- sums
     for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
-      const int64_t b = p.geo.cu ? 0 : t.n;
-      double x[4], sum = 0.0;
+      // this lane's four tokens of a chunk lie `gs` bytes apart (0: one decay for all)
+      const int es = p.dec.dtype == GDN2_BF16 ? 2 : 4;
+      const bool token = p.dec.kind == GDN2_DECAY_TOKEN;
+      const int64_t gs = token ? p.dec.st * es : 0;
+      const char* g0 = static_cast<const char*>(p.dec.g) +
+                       (t.hv * p.dec.sh + (token ? (p.geo.cu ? t.bos * p.dec.st : t.n * p.dec.sb) : 0)) * es;
+      uint32_t raw[4];
+      double sum = 0.0;
       auto load = [&](int c) {
-        const int L = rows(c);
-        const int64_t t0 = (p.geo.cu ? t.bos : 0) + (int64_t)c * kC;
+        const int left = p.dec.kind == GDN2_DECAY_NONE ? 0 : rows(c) - 4 * lane;
+        const char* g = g0 + ((int64_t)c * kC + 4 * lane) * gs;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = 4 * lane + e < L ? p.dec.at(b, t0 + 4 * lane + e, t.hv) : 0.0;
+        for (int e = 0; e < 4; ++e)
+          raw[e] = e >= left ? 0
+                   : es == 2 ? *reinterpret_cast<const uint16_t*>(g + e * gs) : *reinterpret_cast<const uint32_t*>(g + e * gs);
       };
       const int nloc = t.ce - t.cb;
       if (nloc > 0) load(nth(0));
       for (int i = 0; i < nloc; ++i, ++it) {
-        const int s = it & 1, L = rows(nth(i));
-        double G[4] = {x[0], x[0] + x[1], 0.0, 0.0};
-        G[2] = G[1] + x[2];
-        G[3] = G[2] + x[3];
+        const int s = it & 1;
+        double G[4];
+        G[0] = p.dec.value(raw[0]);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) G[e] = G[e - 1] + p.dec.value(raw[e]);
+        if (i + 1 < nloc) load(nth(i + 1));  // in flight until the next turn
         double inc = G[3];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -287,201 +356,195 @@ la_scan_kernel(const ScanArgs p, const __grid_constant__ CUtensorMap tmX, const 
           if (lane >= o) inc += y;
         }
         const double before = __shfl_up_sync(0xffffffffu, inc, 1);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) G[e] += lane ? before : 0.0;
-        const double GC = __shfl_sync(0xffffffffu, inc, 31);
-        double ref[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) ref[w] = __shfl_sync(0xffffffffu, G[0], 8 * w);
-        sum += GC;
-        if (i + 1 < nloc) load(nth(i + 1));
-        if (it >= 2 && !(ok = warp_wait(&sm.f_empty[s], ((it >> 1) & 1) ^ 1))) break;
-        Factors& f = sm.f[s];
-        const int own = lane >> 3;
+        float hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int j = 4 * lane + e;
-          f.yw[j] = j >= L ? 0.f : kBack ? p.a.scale * expf((float)G[e]) : expf((float)(GC - G[e]));
-          if constexpr (kOut) {
-            double rw = ref[0];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) rw = own == w ? ref[w] : rw;
-            f.rowE[j] = expf((float)G[e]);
-            f.r[j] = expf((float)(G[e] - rw));
-            f.g2[j] = (float)(G[e] - rw) * kLog2e;
-#pragma unroll
-            for (int w = 1; w < 4; ++w)
-              if (own < w) f.cf[w - 1][j] = expf((float)(ref[w] - G[e]));
-          }
+          G[e] += lane ? before : 0.0;
+          hi[e] = (float)G[e];
+          lo[e] = (float)(G[e] - (double)hi[e]);
         }
-        if (lane == 0) f.total = expf((float)GC);
+        if (p.pre) sum += __shfl_sync(0xffffffffu, inc, 31);
+        if (it >= 2 && !(ok = warp_wait(&sm.f_empty[s], ((it >> 1) & 1) ^ 1))) break;
+        reinterpret_cast<float4*>(sm.f[s].hi)[lane] = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        reinterpret_cast<uint2*>(sm.f[s].lo)[lane] = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
         tc::mbar_arrive(&sm.f_full[s]);
       }
       if (p.pre && lane == 0 && t.z == 0) p.seg.D[t.entry * p.a.HV + t.hv] = expf((float)sum);
     }
   } else if (warp == 3) {
     // --------------------------------------------------------------- stores
-    if (lane == 0 && (kOut || kStore)) {
+    if (lane == 0 && kStore) {
       for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
-        if (!get_task<kBack>(p, id, t)) continue;
-        const int b = p.geo.cu ? 0 : (int)t.n;
+        if (!find_task<kBack>(p, id, t)) continue;
         for (int i = 0; i < t.ce - t.cb; ++i, ++it) {
-          const int c = nth(i);
-          if constexpr (kStore) {
-            if (!(ok = tc::mbar_wait(&sm.s_full, it & 1))) break;
-            tc::tma_store_2d(&tmS, sm.S, 64 * t.z, (int)(((t.chunk0 + c) * p.a.HV + t.hv) * K));
-            tc::bulk_commit();
-            tc::bulk_wait_read_all();
-            tc::mbar_arrive(&sm.s_free);
-          }
-          if constexpr (kOut) {
-            if (!(ok = tc::mbar_wait(&sm.o_staged[it & 1], (it >> 1) & 1))) break;
-            if (!p.geo.cu || rows(c) == kC) {  // (the last rows of a packed sequence: stored by their threads)
-              tc::tma_store_4d(&tmO, sm.Y[it & 1], 64 * t.z, (int)t.hv, tok(c), b);
-              tc::bulk_commit();
-              tc::bulk_wait_read_all();
-            }
-            tc::mbar_arrive(&sm.empty_y[it & 1]);
-          }
+          if (!(ok = wait(&sm.s_full, it & 1))) break;
+          tc::tma_store_2d(&tmS, sm.S, 64 * t.z, (int)(((t.chunk0 + nth(i)) * p.a.HV + t.hv) * K));
+          tc::bulk_commit();
+          tc::bulk_wait_read_all();
+          tc::mbar_arrive(&sm.s_free);
         }
       }
       tc::bulk_wait_all();
     }
-  } else if (kOut && warp < 8) {
+  } else if (kOut && warp < 12) {
     // --------------------------------------------------------------- scores
-    const int w = warp - 4, i = 32 * w + lane;
+    const int w = warp & 3, i = 32 * w + lane, p2 = (warp - 4) >> 2;  // columns 64 p2 .. 64 p2 + 63
     for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
       for (int j = 0; j < t.ce - t.cb; ++j, ++it) {
         const int s = it & 1;
-        const uint32_t tp = tb + kColQK + 128 * s + ((uint32_t)(32 * w) << 16);
-        if (!(ok = warp_wait(&sm.f_full[s], (it >> 1) & 1) && warp_wait(&sm.qk_full[s], (it >> 1) & 1))) break;
+        const uint32_t tp = tb + kColQK + 128 * s + 64 * p2 + ((uint32_t)(32 * w) << 16);
+        if (!(ok = warp_wait(&sm.f_full[s], (it >> 1) & 1))) break;
+        const Sums& f = sm.f[s];
+        const float gi = sum_diff(f, i, 32 * w) * kLog2e;
+        float* cw = sm.cw + 16 * w * (w + 1);  // (both warps with this w: each its own columns)
+        if (64 * p2 < 32 * w) cw[64 * p2 + lane] = exp2_approx(sum_diff(f, 32 * w, 64 * p2 + lane) * kLog2e);
+        if (64 * p2 + 32 < 32 * w) cw[64 * p2 + 32 + lane] = exp2_approx(sum_diff(f, 32 * w, 64 * p2 + 32 + lane) * kLog2e);
+        if (p2 == w >> 1) cw[i] = gi;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
+        const float ri = exp2_approx(gi);
+        const uint64_t ri2 = tc::pack2(ri, ri);
+        if (!(ok = warp_wait(&sm.qk_full[s], (it >> 1) & 1))) break;
         tc::tc_fence_after();
-        const Factors& f = sm.f[s];
-        const float ri = f.r[i], gi = f.g2[i];
 #pragma unroll 1
-        for (int J = 0; J < 4; ++J) {
-          uint32_t pk[16];
-          if (J > w) {
+        for (int b = 0; b < 4; ++b) {  // 16 columns a turn: a short loop stays in the instruction cache
+          const int c0 = 64 * p2 + 16 * b, d0 = c0 - 32 * w;  // first column, and its place in the diagonal block
+          const float4* cc = reinterpret_cast<const float4*>(cw + c0);
+          uint32_t pk[8];
+          if (d0 >= 32) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = 0;
+            for (int e = 0; e < 8; ++e) pk[e] = 0;
           } else {
-            float x[32];
-            tc::tmem_ld32(tp + 32 * J, x);
-            if (J < w) {
-              const float4* cf = reinterpret_cast<const float4*>(f.cf[w - 1] + 32 * J);
-              tc::tmem_wait_ld();
+            float x[16];
+            tc::tmem_ld16(tp + 16 * b, x);
+            tc::tmem_wait_ld();
+            if (d0 < 0) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float4 cc = cf[e];
-                pk[2 * e] = pack_bf16(x[4 * e] * cc.x * ri, x[4 * e + 1] * cc.y * ri);
-                pk[2 * e + 1] = pack_bf16(x[4 * e + 2] * cc.z * ri, x[4 * e + 3] * cc.w * ri);
+              for (int e = 0; e < 4; ++e) {
+                const float4 c = cc[e];
+                float y[4];
+                tc::unpack2(tc::mul2(tc::mul2(tc::pack2(x[4 * e], x[4 * e + 1]), tc::pack2(c.x, c.y)), ri2), y[0], y[1]);
+                tc::unpack2(tc::mul2(tc::mul2(tc::pack2(x[4 * e + 2], x[4 * e + 3]), tc::pack2(c.z, c.w)), ri2), y[2],
+                            y[3]);
+                pk[2 * e] = pack_bf16(y[0], y[1]);
+                pk[2 * e + 1] = pack_bf16(y[2], y[3]);
               }
             } else {
-              const float4* gj = reinterpret_cast<const float4*>(f.g2 + 32 * J);
-              tc::tmem_wait_ld();
+              const int last = lane - d0;  // columns up to this one are not in the future
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float4 gg = gj[e];
-                const float d[4] = {gg.x, gg.y, gg.z, gg.w};
+              for (int e = 0; e < 4; ++e) {
+                const float4 c = cc[e];
+                const float d[4] = {c.x, c.y, c.z, c.w};
                 float y[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) y[u] = 4 * e + u <= lane ? x[4 * e + u] * exp2_approx(gi - d[u]) : 0.f;
+                for (int u = 0; u < 4; ++u) y[u] = 4 * e + u <= last ? x[4 * e + u] * exp2_approx(gi - d[u]) : 0.f;
                 pk[2 * e] = pack_bf16(y[0], y[1]);
                 pk[2 * e + 1] = pack_bf16(y[2], y[3]);
               }
             }
           }
-          tc::tmem_st16(tp + 16 * J, pk);
+          tc::tmem_st8(tp + 8 * b, pk);
         }
         tc::tmem_wait_st();
         tc::tc_fence_before();
         tc::mbar_arrive(&sm.p_full[s]);
-        if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
       }
     }
-  } else if (kOut ? warp < 12 : warp >= 4 && warp < 8) {
+  } else if (kOut ? warp < 16 : warp >= 4) {
     // ---------------------------------------------------------------- state
     const int w = warp & 3, row = K == 128 ? 32 * w + lane : 16 * w + (lane & 15), j = 32 * w + lane;
     const bool own = K == 128 || lane < 16;  // M = 64: rows in the first 16 lanes of each quarter
     const uint32_t td = tb + kColDS + ((uint32_t)(32 * w) << 16);
     float st[64];
-    uint32_t done = 0;   // chunks whose state term has been taken
+    float total[2];  // e^{G_C} of the last chunks, by parity
     // w v of chunk `it`
     auto weigh = [&](int c) -> bool {
       const int s = it & 1, L = rows(c);
-      if (!warp_wait(&sm.f_full[s], (it >> 1) & 1) || !warp_wait(&sm.full_y[s], (it >> 1) & 1)) return false;
-      char* src = reinterpret_cast<char*>(sm.Y[s]) + j * 128;
-      char* hi = reinterpret_cast<char*>(sm.YW[kNB == 2 ? s : 0]) + j * 128;
-      char* lo = reinterpret_cast<char*>(sm.YW[1]) + j * 128;
-      const float f = sm.f[s].yw[j];
-      const bool inside = j < L;
-#pragma unroll
+      const uint32_t sy = it % NY, b = it % NB;
+      if (!warp_wait(&sm.f_full[s], (it >> 1) & 1)) return false;
+      const float f = j >= L ? 0.f : kBack ? p.a.scale * exp_of(sm.f[s].hi[j]) : exp_of(sum_diff(sm.f[s], kC - 1, j));
+      const float tot = exp_of(sm.f[s].hi[kC - 1] + __bfloat162float(sm.f[s].lo[kC - 1]));
+      if (s) total[1] = tot;
+      else total[0] = tot;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
+      const uint32_t fh = pack_bf16(f, f);
+      const float fr = f - bf16_round(f);
+      const uint32_t fl = pack_bf16(fr, fr);
+      if (!warp_wait(&sm.full_y[sy], (it / NY) & 1)) return false;
+      char* src = reinterpret_cast<char*>(sm.Y[sy]) + j * 128;
+      char* hi = reinterpret_cast<char*>(sm.YW[b][0]) + j * 128;
+      char* lo = reinterpret_cast<char*>(sm.YW[b][kExact ? 1 : 0]) + j * 128;
+#pragma unroll 2
       for (int q = 0; q < 8; ++q) {
         const int at = (q ^ (j & 7)) << 4;
-        float x[8];
-        ld8(reinterpret_cast<const __nv_bfloat16*>(src + at), x);
+        const uint4 v4 = *reinterpret_cast<const uint4*>(src + at);
+        const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
+        uint32_t h[4], l[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = inside ? x[e] * f : 0.f;
-        const uint4 h = pack8(x);
-        *reinterpret_cast<uint4*>(hi + at) = h;
-        if constexpr (kExact) {
-          float y[8];
-          ld8(reinterpret_cast<const __nv_bfloat16*>(&h), y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] -= y[e];
-          *reinterpret_cast<uint4*>(lo + at) = pack8(x);
+        for (int e = 0; e < 4; ++e) {
+          h[e] = tc::bmul2(v[e], fh);
+          // what the product of the leading parts lost (exact), and the trailing part's product
+          if constexpr (kExact) l[e] = tc::bfma2(v[e], fl, tc::bfma2(v[e], fh, h[e] ^ 0x80008000u));
         }
+        *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        if constexpr (kExact) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
       }
       if (p.geo.cu && L < kC) {  // the next sequence's rows in this tile: none of them may reach a sum
-        if (!warp_wait(&sm.full_x[s], (it >> 1) & 1)) return false;
-        if (!inside) {
-#pragma unroll
+        if (!warp_wait(&sm.full_x[it % NX], (it / NX) & 1)) return false;
+        if (j >= L) {
+#pragma unroll 1
           for (int q = 0; q < 8; ++q) {
             *reinterpret_cast<uint4*>(src + 16 * q) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(hi + 16 * q) = make_uint4(0, 0, 0, 0);
+            if constexpr (kExact) *reinterpret_cast<uint4*>(lo + 16 * q) = make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int b = 0; b < K / 64; ++b)
-              *reinterpret_cast<uint4*>(reinterpret_cast<char*>(sm.X[s][b]) + j * 128 + 16 * q) = make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < K / 64; ++e)
+              *reinterpret_cast<uint4*>(reinterpret_cast<char*>(sm.X[it % NX][e]) + j * 128 + 16 * q) =
+                  make_uint4(0, 0, 0, 0);
           }
         }
       }
       tc::fence_proxy_async();
-      tc::mbar_arrive(&sm.yw_full[s]);
-      if constexpr (!kOut) tc::mbar_arrive(&sm.empty_y[s]);
+      tc::mbar_arrive(&sm.yw_full[b]);
+      if constexpr (!kOut) tc::mbar_arrive(&sm.empty_y[sy]);
       return true;
     };
-    // S <- total S + the term of chunk `done`
-    auto take = [&]() -> bool {
-      const int s = done & 1;
-      const float f = sm.f[s].total;
-      if (!warp_wait(&sm.ds_full[s], (done >> 1) & 1)) return false;
+    // S <- total S + the term of chunk d
+    auto take = [&](uint32_t d) -> bool {
+      const uint32_t b = d % NB;
+      const float f = (d & 1) ? total[1] : total[0];
+      const uint64_t f2 = tc::pack2(f, f);
+      if (!warp_wait(&sm.ds_full[b], (d / NB) & 1)) return false;
       tc::tc_fence_after();
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float x[32];
-        tc::tmem_ld32(td + 64 * s + 32 * h, x);
+      for (int h = 0; h < 4; ++h) {
+        float x[16];
+        tc::tmem_ld16(td + 64 * b + 16 * h, x);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) st[32 * h + e] = fmaf(st[32 * h + e], f, x[e]);
+        for (int e = 0; e < 16; e += 2) {
+          float* y = st + 16 * h + e;
+          tc::unpack2(tc::fma2(tc::pack2(y[0], y[1]), f2, tc::pack2(x[e], x[e + 1])), y[0], y[1]);
+        }
       }
       tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
-      ++done;
       return true;
     };
     // the bf16 state of chunk `it`
     auto publish = [&]() -> bool {
-      if constexpr (kS16) {
-        if (kStore && it > 0 && !warp_wait(&sm.s_free, (it - 1) & 1)) return false;
-        char* dst = reinterpret_cast<char*>(sm.S) + row * 128;
-        if (own) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(dst + ((q ^ (row & 7)) << 4)) = pack8(st + 8 * q);
-        }
-        tc::fence_proxy_async();
-        tc::mbar_arrive(&sm.s_full);
+      if (kStore && it > 0 && !warp_wait(&sm.s_free, (it - 1) & 1)) return false;
+      if constexpr (kOut) {  // Q S of the chunk before is done
+        if (it > 0 && !warp_wait(&sm.empty_x[(it - 1) % NX], ((it - 1) / NX) & 1)) return false;
       }
+      char* dst = reinterpret_cast<char*>(sm.S) + row * 128;
+      if (own) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(dst + ((q ^ (row & 7)) << 4)) = pack8(st + 8 * q);
+      }
+      tc::fence_proxy_async();
+      tc::mbar_arrive(&sm.s_full);
       return true;
     };
     for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
@@ -497,13 +560,19 @@ la_scan_kernel(const ScanArgs p, const __grid_constant__ CUtensorMap tmX, const 
       }
       const int nloc = t.ce - t.cb;
       for (int i = 0; i < nloc; ++i, ++it) {
-        // with two buffers the next w v is made while the MMA of the chunk before still runs
-        if (kNB == 2 && !(ok = weigh(nth(i)))) break;
-        if (i > 0 && !(ok = take())) break;
-        if (!(ok = publish())) break;
-        if (kNB == 1 && !(ok = weigh(nth(i)))) break;
+        // (two buffers: the next w v is made while the MMA of the chunk before still runs)
+        if constexpr (NB == 2) {
+          if (!(ok = weigh(nth(i)))) break;
+        }
+        if (i > 0 && !(ok = take(it - 1))) break;
+        if constexpr (NB == 1) {
+          if (!(ok = weigh(nth(i)))) break;
+        }
+        if constexpr (kOut || kStore) {
+          if (!(ok = publish())) break;
+        }
       }
-      if (ok && nloc > 0) ok = take();
+      if (ok && nloc > 0) ok = take(it - 1);
       if (!ok) break;
       float* dst = p.pre ? p.seg.X + (t.entry * p.a.HV + t.hv) * KV
                    : t.tail && p.fin ? p.fin + (t.n * p.a.HV + t.hv) * KV : nullptr;
@@ -513,7 +582,7 @@ la_scan_kernel(const ScanArgs p, const __grid_constant__ CUtensorMap tmX, const 
           *reinterpret_cast<float4*>(dst + at + 4 * q) = make_float4(st[4 * q], st[4 * q + 1], st[4 * q + 2], st[4 * q + 3]);
       }
     }
-  } else if (kOut && warp >= 12) {
+  } else if (kOut) {
     // --------------------------------------------------------------- output
     const int w = warp & 3, i = 32 * w + lane;
     const uint32_t to = tb + ((uint32_t)(32 * w) << 16);
@@ -522,37 +591,27 @@ la_scan_kernel(const ScanArgs p, const __grid_constant__ CUtensorMap tmX, const 
       for (int j = 0; j < t.ce - t.cb; ++j, ++it) {
         const int s = it & 1, c = nth(j), L = rows(c);
         if (!(ok = warp_wait(&sm.f_full[s], (it >> 1) & 1))) break;
-        const float f = sm.f[s].rowE[i];
+        const float f = p.a.scale * exp_of(sm.f[s].hi[i]);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
+        const uint64_t f2 = tc::pack2(f, f), sc2 = tc::pack2(p.a.scale, p.a.scale);
+        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.a.o) +
+                             ((t.bos + (int64_t)c * kC + i) * p.a.HV + t.hv) * p.a.V + 64 * t.z;
         if (!(ok = warp_wait(&sm.o_full, it & 1))) break;
         tc::tc_fence_after();
-        uint4 out[8];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[32], y[32];
-          tc::tmem_ld32(to + kColO1 + 32 * h, x);
-          tc::tmem_ld32(to + kColO2 + 32 * h, y);
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          float x[16], y[16];
+          tc::tmem_ld16(to + kColO1 + 64 * s + 16 * h, x);
+          tc::tmem_ld16(to + kColO2 + 16 * h, y);
           tc::tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = p.a.scale * fmaf(f, x[e], y[e]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) out[4 * h + q] = pack8(x + 8 * q);
+          for (int e = 0; e < 16; e += 2)
+            tc::unpack2(tc::fma2(f2, tc::pack2(x[e], x[e + 1]), tc::mul2(sc2, tc::pack2(y[e], y[e + 1]))), x[e], x[e + 1]);
+          if (i < L) st_32bytes(dst + 16 * h, pack8(x), pack8(x + 8));
         }
         tc::tc_fence_before();
         tc::mbar_arrive(&sm.o_free);
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
-        if (!p.geo.cu || L == kC) {
-          char* dst = reinterpret_cast<char*>(sm.Y[s]) + i * 128;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(dst + ((q ^ (i & 7)) << 4)) = out[q];
-          tc::fence_proxy_async();
-        } else if (i < L) {
-          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.a.o) +
-                               ((t.bos + (int64_t)c * kC + i) * p.a.HV + t.hv) * p.a.V + 64 * t.z;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(dst + 8 * q) = out[q];
-        }
-        tc::mbar_arrive(&sm.o_staged[s]);
       }
     }
   }
@@ -631,17 +690,17 @@ bool state_map(CUtensorMap* m, const void* base, int64_t V, int64_t rows, int64_
 }
 
 struct ScanMaps {
-  CUtensorMap x, q, y, o, s;
+  CUtensorMap x, q, y, s;
 };
 
 template <int K, bool kOut, bool kStore, bool kBack, bool kExact>
 int run_scan(const ScanArgs& p, const ScanMaps& m, cudaStream_t s) {
   auto kern = la_scan_kernel<K, kOut, kStore, kBack, kExact>;
-  constexpr size_t bytes = sizeof(ScanSmem<K, kOut>) + 1024;
+  constexpr size_t bytes = sizeof(ScanSmem<K, kOut, kExact>);
   static_assert(bytes <= 227 * 1024, "shared memory of the scan");
   GDN2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
   ProfScope ps(kOut ? kKLinAttnScan : kKLinAttnStates, s);
-  kern<<<(unsigned)std::min<int64_t>(p.tasks, kLaSms), kOut ? 512 : 256, bytes, s>>>(p, m.x, m.q, m.y, m.o, m.s);
+  kern<<<(unsigned)std::min<int64_t>(p.tasks, kLaSms), kOut ? 640 : 256, bytes, s>>>(p, m.x, m.q, m.y, m.s);
   GDN2_LAUNCH_CHECK();
   return 0;
 }
@@ -673,13 +732,13 @@ int la_tc_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_
   ScanArgs p{a, la_decay(a), la_geom(a, ws), la_segs(a, ws.seg), 0, 0, (a.flags & GDN2_HAS_H0) ? a.h0 : nullptr,
              (a.flags & GDN2_STORE_FINAL) ? a.ht : nullptr};
   p.tasks = p.seg.entries * a.HV * (a.V / 64);
+  if (p.tasks >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
   const bool save = a.flags & GDN2_SAVE_FOR_BWD;
   ScanMaps m;
-  const int64_t ostep[3] = {a.T * a.HV * a.V, a.HV * a.V, a.V};
   if (!token_map(&m.x, a.k, a.K, a.H, a.T, a.B, a.k_stride) || !token_map(&m.q, a.q, a.K, a.H, a.T, a.B, a.q_stride) ||
-      !token_map(&m.y, a.v, a.V, a.HV, a.T, a.B, a.v_stride) || !token_map(&m.o, a.o, a.V, a.HV, a.T, a.B, ostep))
+      !token_map(&m.y, a.v, a.V, a.HV, a.T, a.B, a.v_stride))
     return GDN2_ERR_TENSOR_MAP;
-  m.s = m.o;
+  m.s = m.y;
   if (save && !state_map(&m.s, ws.states16, a.V, la_num_chunks(a) * a.HV * a.K, a.K)) return GDN2_ERR_TENSOR_MAP;
   const bool exact = a.flags & GDN2_STORE_FINAL;
   return a.K == 128 ? scan<128, false>(p, m, true, save, exact, s) : scan<64, false>(p, m, true, save, exact, s);
