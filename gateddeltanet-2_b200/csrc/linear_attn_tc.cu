@@ -19,9 +19,10 @@
 //               e^{G_i - G_r} e^{G_r - G_j} with r the first row of the 32-row block:
 //               both factors are at most 1 for decays, one is per row, the other per
 //               block and column, so only the 32 diagonal columns take an exponential each.
-//   warps 12-15 w v in bf16, and the state in registers (thread = row k of S):
-//               S <- e^{G_C} S + what the MMA left in TMEM; bf16 copy for Q S
-//   warps 16-19 o out of TMEM (thread = token), straight to memory, 32 bytes a store
+//   warps 12-15 half of w v in bf16, and the state in registers (thread = row k of
+//               S): S <- e^{G_C} S + what the MMA left in TMEM; bf16 copy for Q S
+//   warps 16-19 the other half of w v; o out of TMEM (thread = token), straight to
+//               memory, 32 bytes a store
 // MMA order per chunk i: Q K^T, K^T (w v), then P V of chunk i - 1, then Q S.  The
 // lag gives the scores more than a chunk's time, and a q, k stage is held only
 // from its first product to its last, so two stages cover the loads' latency.
@@ -34,6 +35,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "linear_attn.cuh"
 #include "profile.cuh"
@@ -202,7 +204,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       tc::mbar_init(&sm.p_full[i], 256);
     }
     for (uint32_t i = 0; i < NB; ++i) {
-      tc::mbar_init(&sm.yw_full[i], 128);
+      tc::mbar_init(&sm.yw_full[i], kOut ? 256 : 128);
       tc::mbar_init(&sm.ds_full[i], 1);
     }
     tc::mbar_init(&sm.s_full, 128);
@@ -225,6 +227,68 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
   // the token coordinate and batch of chunk c in the tensor maps
   auto tok = [&](int c) { return (int)((p.geo.cu ? t.bos : 0) + (int64_t)c * kC); };
   const int64_t step = gridDim.x;
+  // w v of chunk `it`, 16-byte pieces q0 .. q0 + nq of this thread's token j.  Returns the chunk's sums it
+  // was made from through f_row (e^{G_j}) and total (e^{G_C}).
+  auto weigh = [&](int c, int j, auto q0, auto nq, float& f_row, float& total) -> bool {
+    const int s = it & 1, L = rows(c);
+    const uint32_t sy = it % NY, b = it % NB;
+    if (!warp_wait(&sm.f_full[s], (it >> 1) & 1)) return false;
+    const Sums& g = sm.f[s];
+    const float hi_j = g.hi[j], last = g.hi[kC - 1] + __bfloat162float(g.lo[kC - 1]);
+    f_row = exp_of(hi_j);
+    total = exp_of(last);
+    const float f = j >= L ? 0.f : kBack ? p.a.scale * f_row : exp_of(sum_diff(g, kC - 1, j));
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
+    const uint32_t fh = pack_bf16(f, f);
+    const float fr = f - bf16_round(f);
+    const uint32_t fl = pack_bf16(fr, fr);
+    char* src = reinterpret_cast<char*>(sm.Y[sy]) + j * 128;
+    char* hi = reinterpret_cast<char*>(sm.YW[b][0]) + j * 128;
+    [[maybe_unused]] char* lo = reinterpret_cast<char*>(sm.YW[b][kExact ? 1 : 0]) + j * 128;
+    if (!warp_wait(&sm.full_y[sy], (it / NY) & 1)) return false;
+    if (NB == 1 && it > 0 && !warp_wait(&sm.ds_full[0], (it - 1) & 1)) return false;  // YW has been read
+#pragma unroll 4
+    for (int q = q0; q < q0 + nq; ++q) {
+      const int at = (q ^ (j & 7)) << 4;
+      const uint4 v4 = *reinterpret_cast<const uint4*>(src + at);
+      const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
+      uint32_t h[4];
+      [[maybe_unused]] uint32_t l[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        h[e] = tc::bmul2(v[e], fh);
+        // what the product of the leading parts lost (exact), and the trailing part's product
+        if constexpr (kExact) l[e] = tc::bfma2(v[e], fl, tc::bfma2(v[e], fh, h[e] ^ 0x80008000u));
+      }
+      *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      if constexpr (kExact) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    if (p.geo.cu && L < kC) {  // the next sequence's rows in this tile: none of them may reach a sum
+      if (!warp_wait(&sm.full_x[it % NX], (it / NX) & 1)) return false;
+      if (j >= L) {
+#pragma unroll 1
+        for (int q = q0; q < q0 + nq; ++q) {
+          const int at = (q ^ (j & 7)) << 4;
+          *reinterpret_cast<uint4*>(src + at) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(hi + at) = make_uint4(0, 0, 0, 0);
+          if constexpr (kExact) *reinterpret_cast<uint4*>(lo + at) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < K / 64; ++e)
+            *reinterpret_cast<uint4*>(reinterpret_cast<char*>(sm.X[it % NX][e]) + j * 128 + at) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    tc::fence_proxy_async();
+    tc::mbar_arrive(&sm.yw_full[b]);
+    if constexpr (!kOut) tc::mbar_arrive(&sm.empty_y[sy]);
+    return true;
+  };
+  using std::integral_constant;
+  const integral_constant<int, 0> kQ0{};
+  const integral_constant<int, 4> kHalf{};
+  const integral_constant<int, 8> kAll{};
+
 
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
@@ -457,65 +521,11 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
     const bool own = K == 128 || lane < 16;  // M = 64: rows in the first 16 lanes of each quarter
     const uint32_t td = tb + kColDS + ((uint32_t)(32 * w) << 16);
     float st[64];
-    float total[2];  // e^{G_C} of the last chunks, by parity
-    // w v of chunk `it`
-    auto weigh = [&](int c) -> bool {
-      const int s = it & 1, L = rows(c);
-      const uint32_t sy = it % NY, b = it % NB;
-      if (!warp_wait(&sm.f_full[s], (it >> 1) & 1)) return false;
-      const float f = j >= L ? 0.f : kBack ? p.a.scale * exp_of(sm.f[s].hi[j]) : exp_of(sum_diff(sm.f[s], kC - 1, j));
-      const float tot = exp_of(sm.f[s].hi[kC - 1] + __bfloat162float(sm.f[s].lo[kC - 1]));
-      if (s) total[1] = tot;
-      else total[0] = tot;
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
-      const uint32_t fh = pack_bf16(f, f);
-      const float fr = f - bf16_round(f);
-      const uint32_t fl = pack_bf16(fr, fr);
-      if (!warp_wait(&sm.full_y[sy], (it / NY) & 1)) return false;
-      char* src = reinterpret_cast<char*>(sm.Y[sy]) + j * 128;
-      char* hi = reinterpret_cast<char*>(sm.YW[b][0]) + j * 128;
-      char* lo = reinterpret_cast<char*>(sm.YW[b][kExact ? 1 : 0]) + j * 128;
-#pragma unroll 2
-      for (int q = 0; q < 8; ++q) {
-        const int at = (q ^ (j & 7)) << 4;
-        const uint4 v4 = *reinterpret_cast<const uint4*>(src + at);
-        const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[e] = tc::bmul2(v[e], fh);
-          // what the product of the leading parts lost (exact), and the trailing part's product
-          if constexpr (kExact) l[e] = tc::bfma2(v[e], fl, tc::bfma2(v[e], fh, h[e] ^ 0x80008000u));
-        }
-        *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-        if constexpr (kExact) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-      }
-      if (p.geo.cu && L < kC) {  // the next sequence's rows in this tile: none of them may reach a sum
-        if (!warp_wait(&sm.full_x[it % NX], (it / NX) & 1)) return false;
-        if (j >= L) {
-#pragma unroll 1
-          for (int q = 0; q < 8; ++q) {
-            *reinterpret_cast<uint4*>(src + 16 * q) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(hi + 16 * q) = make_uint4(0, 0, 0, 0);
-            if constexpr (kExact) *reinterpret_cast<uint4*>(lo + 16 * q) = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < K / 64; ++e)
-              *reinterpret_cast<uint4*>(reinterpret_cast<char*>(sm.X[it % NX][e]) + j * 128 + 16 * q) =
-                  make_uint4(0, 0, 0, 0);
-          }
-        }
-      }
-      tc::fence_proxy_async();
-      tc::mbar_arrive(&sm.yw_full[b]);
-      if constexpr (!kOut) tc::mbar_arrive(&sm.empty_y[sy]);
-      return true;
-    };
+    float total = 0.f, total_next = 0.f;  // e^{G_C} of the chunk before, of this one
     // S <- total S + the term of chunk d
     auto take = [&](uint32_t d) -> bool {
       const uint32_t b = d % NB;
-      const float f = (d & 1) ? total[1] : total[0];
-      const uint64_t f2 = tc::pack2(f, f);
+      const uint64_t f2 = tc::pack2(total, total);
       if (!warp_wait(&sm.ds_full[b], (d / NB) & 1)) return false;
       tc::tc_fence_after();
 #pragma unroll
@@ -547,9 +557,10 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       tc::mbar_arrive(&sm.s_full);
       return true;
     };
+    const int64_t KV = (int64_t)K * p.a.V;
     for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
-      const int64_t KV = (int64_t)K * p.a.V, at = (int64_t)row * p.a.V + 64 * t.z;
+      const int64_t at = (int64_t)row * p.a.V + 64 * t.z;
       const float* src = t.head ? (p.init ? p.init + (t.n * p.a.HV + t.hv) * KV : nullptr)
                          : p.pre ? nullptr
                                  : p.seg.X + ((t.entry + (kBack ? 1 : -1)) * p.a.HV + t.hv) * KV;
@@ -559,20 +570,23 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
         st[4 * q] = x.x; st[4 * q + 1] = x.y; st[4 * q + 2] = x.z; st[4 * q + 3] = x.w;
       }
       const int nloc = t.ce - t.cb;
-      for (int i = 0; i < nloc; ++i, ++it) {
-        // (two buffers: the next w v is made while the MMA of the chunk before still runs)
-        if constexpr (NB == 2) {
-          if (!(ok = weigh(nth(i)))) break;
+      float unused;
+      for (int i = 0; i <= nloc; ++i) {
+        if constexpr (NB == 2) {  // two buffers: w v before the MMA of the chunk before has ended
+          if (i < nloc && !(ok = weigh(nth(i), j, kQ0, kAll, unused, total_next))) break;
         }
+        // (one buffer: the state term leaves TMEM before this half of w v lets the next one in)
         if (i > 0 && !(ok = take(it - 1))) break;
         if constexpr (NB == 1) {
-          if (!(ok = weigh(nth(i)))) break;
+          if (i < nloc && !(ok = weigh(nth(i), j, kQ0, kHalf, unused, total_next))) break;
         }
+        total = total_next;
+        if (i == nloc) break;
         if constexpr (kOut || kStore) {
           if (!(ok = publish())) break;
         }
+        ++it;
       }
-      if (ok && nloc > 0) ok = take(it - 1);
       if (!ok) break;
       float* dst = p.pre ? p.seg.X + (t.entry * p.a.HV + t.hv) * KV
                    : t.tail && p.fin ? p.fin + (t.n * p.a.HV + t.hv) * KV : nullptr;
@@ -583,37 +597,53 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       }
     }
   } else if (kOut) {
-    // --------------------------------------------------------------- output
+    // ------------------------------------------------------- output, half of w v
+    // Chunk it's half of w v comes before chunk it - 2's output, across tasks
+    // too: the MMAs of chunk it wait for the one and go before the other's end.
     const int w = warp & 3, i = 32 * w + lane;
     const uint32_t to = tb + ((uint32_t)(32 * w) << 16);
+    const uint64_t sc2 = tc::pack2(p.a.scale, p.a.scale);
+    const int64_t chunk_step = (int64_t)kC * p.a.HV * p.a.V;
+    // of chunks it - 2 and it - 1: e^{G_i}, and this thread's row of o (NULL past the sequence's end)
+    float f = 0.f, f1 = 0.f, f_next = 0.f, unused;
+    __nv_bfloat16 *dst = nullptr, *dst1 = nullptr;
+    auto output = [&](uint32_t d) -> bool {
+      if (!warp_wait(&sm.o_full, d & 1)) return false;
+      tc::tc_fence_after();
+      const uint64_t f2 = tc::mul2(sc2, tc::pack2(f, f));
+#pragma unroll 1
+      for (int h = 0; h < 4; ++h) {
+        float x[16], y[16];
+        tc::tmem_ld16(to + kColO1 + 64 * (d & 1) + 16 * h, x);
+        tc::tmem_ld16(to + kColO2 + 16 * h, y);
+        tc::tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; e += 2)
+          tc::unpack2(tc::fma2(f2, tc::pack2(x[e], x[e + 1]), tc::mul2(sc2, tc::pack2(y[e], y[e + 1]))), x[e], x[e + 1]);
+        if (dst) st_32bytes(dst + 16 * h, pack8(x), pack8(x + 8));
+      }
+      tc::tc_fence_before();
+      tc::mbar_arrive(&sm.o_free);
+      return true;
+    };
     for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
+      __nv_bfloat16* const row0 =
+          static_cast<__nv_bfloat16*>(p.a.o) + ((t.bos + i) * p.a.HV + t.hv) * p.a.V + 64 * t.z;
       for (int j = 0; j < t.ce - t.cb; ++j, ++it) {
-        const int s = it & 1, c = nth(j), L = rows(c);
-        if (!(ok = warp_wait(&sm.f_full[s], (it >> 1) & 1))) break;
-        const float f = p.a.scale * exp_of(sm.f[s].hi[i]);
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
-        const uint64_t f2 = tc::pack2(f, f), sc2 = tc::pack2(p.a.scale, p.a.scale);
-        __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.a.o) +
-                             ((t.bos + (int64_t)c * kC + i) * p.a.HV + t.hv) * p.a.V + 64 * t.z;
-        if (!(ok = warp_wait(&sm.o_full, it & 1))) break;
-        tc::tc_fence_after();
-#pragma unroll 1
-        for (int h = 0; h < 4; ++h) {
-          float x[16], y[16];
-          tc::tmem_ld16(to + kColO1 + 64 * s + 16 * h, x);
-          tc::tmem_ld16(to + kColO2 + 16 * h, y);
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; e += 2)
-            tc::unpack2(tc::fma2(f2, tc::pack2(x[e], x[e + 1]), tc::mul2(sc2, tc::pack2(y[e], y[e + 1]))), x[e], x[e + 1]);
-          if (i < L) st_32bytes(dst + 16 * h, pack8(x), pack8(x + 8));
-        }
-        tc::tc_fence_before();
-        tc::mbar_arrive(&sm.o_free);
+        const int c = nth(j);
+        if (!(ok = weigh(c, i, kHalf, kHalf, f_next, unused))) break;
+        if (it > 1 && !(ok = output(it - 2))) break;
+        f = f1;
+        dst = dst1;
+        f1 = f_next;
+        dst1 = i < rows(c) ? row0 + c * chunk_step : nullptr;
       }
     }
+    if (ok && it > 1) ok = output(it - 2);
+    f = f1;
+    dst = dst1;
+    if (ok && it > 0) ok = output(it - 1);
   }
   if (!ok) atomicOr(&g_la_fault, 1u);
   tc::tc_fence_before();
