@@ -55,6 +55,7 @@ struct LaGeom {
 struct LaSegs {
   int len;              // chunks per segment
   bool multi;           // some sequence may have several
+  bool cut;             // packed and cut: the entries are looked up in `map`
   int64_t per;          // segments per sequence (dense)
   int64_t entries;      // segments over all sequences (packed and cut: an upper bound)
   const LaChunk* map;   // [entries] (sequence, segment), packed and cut only
@@ -91,13 +92,13 @@ struct LaWs {
 };
 struct LaBwdWs {
   float* dstates;   // [NT, HV, K, V] fp32 (fp32 kernels)
+  __nv_bfloat16* dstates16;  // [NT, HV, K, V] bf16 (tensor-core kernels)
+  float* acc;       // [CTAs, 2, 128, K] running sums over a group of value heads (tensor-core kernels)
+  LaSegWs seg;
   float* dg;        // [B, T, HV] fp32, the terms of a per-head decay's gradient
 };
 
-// the simple path also runs bf16 training until its backward is on the tensor cores
-inline bool la_tc(const gdn2_linear_attn_args& a) {
-  return a.dtype == GDN2_BF16 && !(a.flags & GDN2_SAVE_FOR_BWD);
-}
+inline bool la_tc(const gdn2_linear_attn_args& a) { return a.dtype == GDN2_BF16; }
 inline int la_chunk(const gdn2_linear_attn_args& a) { return la_tc(a) ? kLaChunkTc : kLaChunkF32; }
 
 // chunks over all sequences: exact for dense batches, an upper bound for packed
@@ -125,6 +126,7 @@ inline LaSegs la_segs(const gdn2_linear_attn_args& a, const LaSegWs& ws) {
   if (g.multi) {
     g.map = a.cu_seqlens ? ws.map : nullptr;
     g.first = ws.first;
+    g.cut = a.cu_seqlens != nullptr;
     g.X = ws.X;
     g.D = ws.D;
   }
@@ -176,7 +178,17 @@ inline size_t la_bwd_ws_layout(const gdn2_linear_attn_args& a, void* base, LaBwd
   };
   LaBwdWs w{};
   const size_t NT = (size_t)la_num_chunks(a), HV = (size_t)a.HV, KV = (size_t)(a.K * a.V);
-  w.dstates = (float*)take(NT * HV * KV * 4);
+  if (la_tc(a)) {
+    const LaSegs g = la_segs(a, w.seg);
+    if (g.multi) {
+      w.seg.X = (float*)take((size_t)g.entries * HV * KV * 4);
+      w.seg.D = (float*)take((size_t)g.entries * HV * 4);
+    }
+    w.dstates16 = (__nv_bfloat16*)take(NT * HV * KV * 2);
+    if (a.HV > a.H) w.acc = (float*)take((size_t)kLaSms * 2 * kLaChunkTc * (size_t)a.K * 4);
+  } else {
+    w.dstates = (float*)take(NT * HV * KV * 4);
+  }
   if (a.decay == GDN2_DECAY_HEAD) w.dg = (float*)take((size_t)(a.B * a.T) * HV * 4);
   if (out) *out = w;
   return off;
@@ -216,6 +228,8 @@ int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& 
 int la_tc_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s);
 // fault word of the tensor-core kernels: bit 0 = a bounded wait gave up
 int la_fault_read(int clear, unsigned int* out);
+int la_tc_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
+                     const LaBwdWs& bw, cudaStream_t s);
 int la_recurrent_launch(const gdn2_linear_attn_args& a, cudaStream_t s);
 
 int layer_norm_fwd_launch(const gdn2_layer_norm_args& a, cudaStream_t s);

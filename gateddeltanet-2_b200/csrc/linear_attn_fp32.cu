@@ -606,10 +606,6 @@ int bwd(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const 
         a, gr, dec, geo, ws.states, bw.dstates, a.decay == GDN2_DECAY_HEAD ? bw.dg : nullptr);
     GDN2_LAUNCH_CHECK();
   }
-  if (gr.dg && a.decay == GDN2_DECAY_HEAD) {
-    la_head_sum_kernel<<<HV, 256, 0, s>>>(bw.dg, a.B * a.T, HV, gr.dg, a.dtype_g, geo);
-    GDN2_LAUNCH_CHECK();
-  }
   return 0;
 }
 
@@ -665,8 +661,7 @@ int la_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s
     return 0;
   }
   if (la_tc(a)) return la_tc_fwd_launch(a, ws, s);
-  const FwdCall f{a, ws, s};
-  return a.dtype == GDN2_F32 ? by_dims<float>(a, f) : by_dims<__nv_bfloat16>(a, f);
+  return by_dims<float>(a, FwdCall{a, ws, s});
 }
 
 int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
@@ -687,8 +682,16 @@ int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& 
                                               la_geom(a, ws));
     GDN2_LAUNCH_CHECK();
   }
-  const BwdCall f{a, gr, ws, bw, s};
-  return a.dtype == GDN2_F32 ? by_dims<float>(a, f) : by_dims<__nv_bfloat16>(a, f);
+  if (la_tc(a)) {
+    if (int st = la_tc_bwd_launch(a, gr, ws, bw, s)) return st;
+  } else if (int st = by_dims<float>(a, BwdCall{a, gr, ws, bw, s})) {
+    return st;
+  }
+  if (gr.dg && a.decay == GDN2_DECAY_HEAD) {
+    la_head_sum_kernel<<<(unsigned)a.HV, 256, 0, s>>>(bw.dg, a.B * a.T, (int)a.HV, gr.dg, a.dtype_g, la_geom(a, ws));
+    GDN2_LAUNCH_CHECK();
+  }
+  return 0;
 }
 
 }  // namespace gdn2

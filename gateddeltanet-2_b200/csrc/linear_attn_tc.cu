@@ -675,6 +675,556 @@ __global__ void __launch_bounds__(128) la_segment_kernel(LaSegs seg, LaGeom geo,
   }
 }
 
+// sum of 8 products of bf16 pairs
+GDN2_DEV float dot8(const uint4& a, const uint4& b) {
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), s);
+    t = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), t);
+  }
+  return s + t;
+}
+// 16 bf16 of a swizzled row (pieces p0, p0 + 1) times 16 floats
+GDN2_DEV float dot16(const unsigned char* row_base, int p0, int row, const float (&y)[16]) {
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row_base + (((p0 + h) ^ (row & 7)) << 4));
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s = fmaf(__uint_as_float(x[i] << 16), y[8 * h + 2 * i], s);
+      t = fmaf(__uint_as_float(x[i] & 0xffff0000u), y[8 * h + 2 * i + 1], t);
+    }
+  }
+  return s + t;
+}
+
+// ---------------------------------------------------------------------------
+// Backward, one chunk of 128 tokens and one value head at a time (all chunks in
+// parallel), from the chunk's entering state S and leaving cotangent dS':
+//     P^T_ji = scale e^{G_i - G_j} (k_j . q_i),  E^T_ji = scale e^{G_i - G_j} (v_j . do_i)   (i >= j)
+//     dq = scale e^G do S^T + E k      dk = e^{G_C - G} v dS'^T + E^T q      dv = e^{G_C - G} k dS' + P^T do
+// Nine products of M = 128 tokens.  The scores come out transposed (rows j), so
+// that P^T and E^T are TMEM operands of dv and dk as they are; E^T also goes to
+// shared memory, where it is the M-major operand of dq.  The products with the
+// states land in the gradients' accumulators first; their rows are scaled
+// there, then the products within the chunk add to them.
+// dg: with X_i = q_i . dq_i and Y_j = k_j . dk_j (fp32, before rounding), whose parts from within the
+// chunk use the same bf16 E and so cancel where they must,
+//     dg_t = sum_{i>=t} (X_i - Y_i) + sum_j k_j . (e^{G_C - G_j} v_j dS'^T) + e^{G_C} <S, dS'>.
+// A sequence's first token without an initial state decays nothing: exactly zero.
+// Shared memory holds one chunk's six tiles and E^T; a tile's slot goes to the
+// next chunk's tile (x + 3) % 6 as soon as it has been read, so v, S and dS' make
+// room for q, k and do of the next chunk while this one is being finished.
+//   warp 0 loads, warp 1 MMAs, warp 2 running sums, warp 3 dg,
+//   warps 4-11: thread = token (TMEM lane) and one half of the columns
+// ---------------------------------------------------------------------------
+enum Tile { kTQ = 0, kTK, kTO, kTV, kTS, kTD };  // q, k, do, v, S, dS'
+
+struct alignas(1024) BwdSmem {
+  __nv_bfloat16 slot[6][128 * 128];
+  __nv_bfloat16 E[2][128 * 64];  // E^T, rows j
+  float hi[kC];                  // running sums of g
+  float g2[kC];                  // (G_i - G_{32 floor(i / 32)}) log2 e
+  float r[kC];                   // 2^g2
+  float xy[2][kC];               // X - Y, per half of the columns
+  float part[16];                // per warp: sum of k . dk (state part), e^{G_C} <S, dS'>
+  uint64_t full[6], empty[6], f_full, f_empty, clean, g1, g2_, pe, rmw1, g3, rmw2, g4a, g4b, qk_free, dv_free, xy_full,
+      xy_free, aborted;
+  uint32_t tbase;
+};
+
+struct BwdArgs {
+  gdn2_linear_attn_args a;
+  gdn2_linear_attn_grads gr;
+  LaDecay dec;
+  LaGeom geo;
+  int64_t items;  // chunks (bound) x key heads
+  float* acc;     // [CTAs, 2, 128, K] running sums of dq, dk over a group of value heads
+  float* dgf;     // [B, T, HV] fp32 terms of a per-head decay's gradient, or NULL
+};
+
+template <int K, int V, bool kDg>
+__global__ void __launch_bounds__(384, 1)
+la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUtensorMap tmQ,
+                 const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmS,
+                 const __grid_constant__ CUtensorMap tmD) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  BwdSmem& sm = *reinterpret_cast<BwdSmem*>(smem_raw);
+  constexpr uint32_t kColA1 = 0, kColA2 = 128, kColDq = 256, kColDk = 384;  // dv: over A2
+  const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < 6; ++i) {
+      tc::mbar_init(&sm.full[i], 1);
+      tc::mbar_init(&sm.empty[i], 9);  // the MMAs' commit and the eight row warps
+    }
+    tc::mbar_init(&sm.f_full, 32);
+    tc::mbar_init(&sm.f_empty, 8);
+    tc::mbar_init(&sm.clean, 256);
+    tc::mbar_init(&sm.g1, 1);
+    tc::mbar_init(&sm.g2_, 1);
+    tc::mbar_init(&sm.pe, 256);
+    tc::mbar_init(&sm.rmw1, 256);
+    tc::mbar_init(&sm.g3, 1);
+    tc::mbar_init(&sm.rmw2, 256);
+    tc::mbar_init(&sm.g4a, 1);
+    tc::mbar_init(&sm.g4b, 1);
+    tc::mbar_init(&sm.qk_free, 256);
+    tc::mbar_init(&sm.dv_free, 256);
+    tc::mbar_init(&sm.xy_full, 256);
+    tc::mbar_init(&sm.xy_free, 32);
+    tc::mbar_init(&sm.aborted, 1);
+    tc::mbar_fence_init();
+  }
+  if (warp == 1) tc::tmem_alloc(&sm.tbase, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tb = sm.tbase;
+  const int group = (int)(p.a.HV / p.a.H);
+  bool ok = true;
+  uint32_t n = 0;  // (chunk, value head) pairs this role has been through
+  struct {
+    int64_t n, c, bos;
+    int h, L;
+  } w{};
+  // item -> sequence, chunk, key head; false past the last chunk
+  auto item = [&](int64_t id) -> bool {
+    const uint32_t H = (uint32_t)p.a.H, ch = (uint32_t)id / H;
+    w.h = (int)((uint32_t)id % H);
+    if (!p.geo.chunk(ch, w.n, w.c)) return false;
+    int64_t len;
+    p.geo.seq(w.n, w.bos, len);
+    w.L = (int)min(len - w.c * kC, (int64_t)kC);
+    return w.L > 0;
+  };
+  auto witem = [&](int64_t id) -> bool {
+    const bool any = __all_sync(0xffffffffu, item(id));
+    w.n = uniform(w.n);
+    w.c = uniform(w.c);
+    w.bos = uniform(w.bos);
+    w.L = uniform(w.L);
+    return any;
+  };
+  auto slot_of = [&](int x) -> int { return (n & 1) ? (x < 3 ? x + 3 : x - 3) : x; };
+  const int64_t step = gridDim.x;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads
+    if (tc::elect_one()) {
+      for (int64_t id = blockIdx.x; id < p.items && ok; id += step) {
+        if (!item(id)) continue;
+        const int b = p.geo.cu ? 0 : (int)w.n, t = (int)((p.geo.cu ? w.bos : 0) + w.c * kC);
+        for (int j = 0; j < group && ok; ++j, ++n) {
+          const int hv = w.h * group + j;
+          const int row = (int)(((p.geo.chunk0(w.n) + w.c) * p.a.HV + hv) * K);
+#pragma unroll 1
+          for (int x = 0; x < 6; ++x) {
+            const int s = slot_of(x);
+            if (n > 0 && !(ok = wait(&sm.empty[s], (n - 1) & 1))) break;
+            unsigned char* dst = reinterpret_cast<unsigned char*>(sm.slot[s]);
+            uint64_t* bar = &sm.full[s];
+            const bool state = x >= kTS, key = x <= kTK;
+            const int blocks = (key ? K : V) / 64;
+            const uint32_t bytes = state ? (uint32_t)K * 128 : kTile;
+            tc::mbar_arrive_expect_tx(bar, blocks * bytes);
+            const CUtensorMap* m = x == kTQ ? &tmQ : x == kTK ? &tmK : x == kTO ? &tmO : x == kTV ? &tmV
+                                                                             : x == kTS ? &tmS : &tmD;
+            for (int c = 0; c < blocks; ++c) {
+              if (state) tc::tma_load_2d(dst + c * bytes, m, bar, 64 * c, row);
+              else tc::tma_load_4d(dst + c * bytes, m, bar, 64 * c, key ? w.h : hv, t, b);
+            }
+          }
+          if (!ok) break;
+        }
+      }
+      if (!ok)  // loads in flight land before the CTA exits, also after a wait that gave up
+        for (int s = 0; s < 6; ++s) {
+          wait(&sm.full[s], n & 1);
+          wait(&sm.full[s], (n + 1) & 1);
+        }
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMAs
+    if (tc::elect_one()) {
+      constexpr uint32_t iA = tc::idesc_bf16(128, 128, 0, 0), iK = tc::idesc_bf16(128, K, 0, 0);
+      constexpr uint32_t iVn = tc::idesc_bf16(128, V, 0, 1), iKn = tc::idesc_bf16(128, K, 0, 1);
+      constexpr uint32_t iKmn = tc::idesc_bf16(128, K, 1, 1);
+      constexpr uint32_t kBlk = K * 128 / 16;  // a state's 64-column block, in 16-byte units
+      const uint32_t a0 = addr16(sm.slot), aE = addr16(sm.E);
+      for (int64_t id = blockIdx.x; id < p.items && ok; id += step) {
+        if (!item(id)) continue;
+        for (int j = 0; j < group; ++j, ++n) {
+          const uint32_t par = n & 1, prev = par ^ 1;
+          auto at = [&](int x) { return a0 + (uint32_t)slot_of(x) * (sizeof(sm.slot[0]) >> 4); };
+          const uint32_t aq = at(kTQ), ak = at(kTK), ao = at(kTO), av = at(kTV), as = at(kTS), ad = at(kTD);
+          auto full = [&](int x) { return wait(&sm.full[slot_of(x)], par); };
+          if (!(ok = full(kTQ) && full(kTK) && wait(&sm.clean, par))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < K / 16; ++kk) tc::mma_bf16(tb + kColA1, kmaj(ak, kk), kmaj(aq, kk), iA, kk > 0);
+          if (!(ok = full(kTO) && full(kTV) && (n == 0 || wait(&sm.dv_free, prev)))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < V / 16; ++kk) tc::mma_bf16(tb + kColA2, kmaj(av, kk), kmaj(ao, kk), iA, kk > 0);
+          tc::mma_commit(&sm.g1);
+          if (!(ok = full(kTS) && (n == 0 || wait(&sm.qk_free, prev)))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < V / 16; ++kk)
+            tc::mma_bf16(tb + kColDq, kmaj(ao, kk), desc(as + (kk >> 2) * kBlk + (kk & 3) * 2 + (1u << 16)), iK, kk > 0);
+          if (!(ok = full(kTD))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < V / 16; ++kk)
+            tc::mma_bf16(tb + kColDk, kmaj(av, kk), desc(ad + (kk >> 2) * kBlk + (kk & 3) * 2 + (1u << 16)), iK, kk > 0);
+          tc::mma_commit(&sm.g2_);
+          tc::mma_commit(&sm.empty[slot_of(kTV)]);
+          tc::mma_commit(&sm.empty[slot_of(kTS)]);
+          if (!(ok = wait(&sm.pe, par))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < K / 16; ++kk)
+            tc::mma_bf16(tb + kColA2, kmaj(ak, kk), desc(ad + kk * 128 + (kBlk << 16)), iVn, kk > 0);
+          tc::mma_commit(&sm.g3);
+          tc::mma_commit(&sm.empty[slot_of(kTD)]);
+          if (!(ok = wait(&sm.rmw1, par))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) tc::mma_bf16(tb + kColDq, nmaj(aE, kk), nmaj(ak, kk), iKmn, 1);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            tc::mma_bf16_ts(tb + kColDk, tb + kColA1 + 64 * (kk >> 2) + 32 + 8 * (kk & 3), nmaj(aq, kk), iKn, 1);
+          tc::mma_commit(&sm.g4a);
+          tc::mma_commit(&sm.empty[slot_of(kTQ)]);
+          tc::mma_commit(&sm.empty[slot_of(kTK)]);
+          if (!(ok = wait(&sm.rmw2, par))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            tc::mma_bf16_ts(tb + kColA2, tb + kColA1 + 64 * (kk >> 2) + 8 * (kk & 3), nmaj(ao, kk), iVn, 1);
+          tc::mma_commit(&sm.g4b);
+          tc::mma_commit(&sm.empty[slot_of(kTO)]);
+        }
+      }
+      tc::mma_commit(&sm.aborted);  // what was issued has completed before TMEM is released
+      if (!wait(&sm.aborted, 0)) ok = false;
+    }
+  } else if (warp == 2) {
+    // ----------------------------------------------------------------- sums
+    for (int64_t id = blockIdx.x; id < p.items && ok; id += step) {
+      if (!witem(id)) continue;
+      const int64_t b = p.geo.cu ? 0 : w.n, t0 = (p.geo.cu ? w.bos : 0) + w.c * kC;
+      for (int j = 0; j < group; ++j, ++n) {
+        double G[4], x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = 4 * lane + e < w.L ? p.dec.at(b, t0 + 4 * lane + e, w.h * group + j) : 0.0;
+        G[0] = x[0];
+#pragma unroll
+        for (int e = 1; e < 4; ++e) G[e] = G[e - 1] + x[e];
+        double inc = G[3];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += y;
+        }
+        const double before = __shfl_up_sync(0xffffffffu, inc, 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) G[e] += lane ? before : 0.0;
+        const double ref = __shfl_sync(0xffffffffu, G[0], lane & 24);  // of this lane's block of 32 tokens
+        float hi[4], g2[4], r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          hi[e] = (float)G[e];
+          g2[e] = (float)(G[e] - ref) * kLog2e;
+          r[e] = exp2_approx(g2[e]);
+        }
+        if (n > 0 && !(ok = warp_wait(&sm.f_empty, (n - 1) & 1))) break;
+        reinterpret_cast<float4*>(sm.hi)[lane] = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        reinterpret_cast<float4*>(sm.g2)[lane] = make_float4(g2[0], g2[1], g2[2], g2[3]);
+        reinterpret_cast<float4*>(sm.r)[lane] = make_float4(r[0], r[1], r[2], r[3]);
+        tc::mbar_arrive(&sm.f_full);
+      }
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------- dg
+    if constexpr (kDg) {
+      for (int64_t id = blockIdx.x; id < p.items && ok; id += step) {
+        if (!witem(id)) continue;
+        for (int j = 0; j < group; ++j, ++n) {
+          if (!(ok = warp_wait(&sm.xy_full, n & 1))) break;
+          const float4 x0 = reinterpret_cast<const float4*>(sm.xy[0])[lane];
+          const float4 x1 = reinterpret_cast<const float4*>(sm.xy[1])[lane];
+          float base = lane < 16 ? sm.part[lane] : 0.f;
+          __syncwarp();
+          tc::mbar_arrive(&sm.xy_free);
+          float d[4] = {x0.x + x1.x, x0.y + x1.y, x0.z + x1.z, x0.w + x1.w};
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
+          // sums from each token to the chunk's end
+#pragma unroll
+          for (int e = 2; e >= 0; --e) d[e] += d[e + 1];
+          float s = d[0];
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const float y = __shfl_down_sync(0xffffffffu, s, o);
+            if (lane + o < 32) s += y;
+          }
+          const float after = s - d[0] + base;
+          const int64_t hv = w.h * group + j;
+          const bool fresh = w.c == 0 && !(p.a.flags & GDN2_HAS_H0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = 4 * lane + e;
+            if (t < w.L) {
+              const float v = fresh && t == 0 ? 0.f : d[e] + after;
+              const int64_t at = (w.bos + w.c * kC + t) * p.a.HV + hv;
+              if (p.dgf) p.dgf[at] = v;
+              else if (p.a.dtype_g == GDN2_BF16) static_cast<__nv_bfloat16*>(p.gr.dg)[at] = __float2bfloat16_rn(v);
+              else static_cast<float*>(p.gr.dg)[at] = v;
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // ----------------------------------------------------------------- rows
+    const int q4 = warp & 3, row = 32 * q4 + lane, half = (warp - 4) >> 2;
+    const uint32_t tl = tb + ((uint32_t)(32 * q4) << 16);
+    const int64_t H = p.a.H, HV = p.a.HV;
+    float* acc = p.acc + ((int64_t)blockIdx.x * 2 * kC + row) * K + half * (K / 2);
+    for (int64_t id = blockIdx.x; id < p.items && ok; id += step) {
+      if (!witem(id)) continue;
+      const int64_t tok = w.bos + w.c * kC + row;
+      const bool inside = row < w.L;
+      for (int j = 0; j < group; ++j, ++n) {
+        const uint32_t par = n & 1;
+        const int hv = w.h * group + j;
+        auto tile = [&](int x) { return reinterpret_cast<unsigned char*>(sm.slot[slot_of(x)]); };
+        auto release = [&](int x) {
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sm.empty[slot_of(x)]);
+        };
+        // rows of the next sequence in these tiles: none of them may reach a sum
+        if (p.geo.cu && w.L < kC) {
+          for (int x = kTQ; x <= kTV; ++x)
+            if (!(ok = warp_wait(&sm.full[slot_of(x)], par))) break;
+          if (!ok) break;
+          if (!inside) {
+#pragma unroll 1
+            for (int x = kTQ; x <= kTV; ++x) {
+              if ((x <= kTK ? K : V) == 64 && half) continue;  // 64-column blocks: one per half
+              uint4* dst = reinterpret_cast<uint4*>(tile(x) + half * kTile + row * 128);
+              for (int e = 0; e < 8; ++e) dst[e] = make_uint4(0, 0, 0, 0);
+            }
+          }
+          tc::fence_proxy_async();
+        }
+        tc::mbar_arrive(&sm.clean);
+        if (!(ok = warp_wait(&sm.f_full, par))) break;
+        const float hj = sm.hi[row], gj = sm.g2[row], gc = sm.hi[kC - 1];
+        const float out_f = p.a.scale * exp_of(hj), in_f = exp_of(gc - hj);  // of the products with S and dS'
+        const float eGC = exp_of(gc);
+        float block_f[2];  // e^{G_{32 I} - G_j} scale of this half's two 32-column blocks (I > q4)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) block_f[e] = p.a.scale * exp_of(sm.hi[64 * half + 32 * e] - hj);
+        if (!(ok = warp_wait(&sm.g1, par))) break;
+        tc::tc_fence_after();
+        // ---- P^T, E^T ------------------------------------------------------
+        {
+          float a1[4][16];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) tc::tmem_ld16(tl + kColA1 + 64 * half + 16 * b, a1[b]);
+          unsigned char* erow = reinterpret_cast<unsigned char*>(sm.E[half]) + row * 128;
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int c0 = 64 * half + 16 * b, d0 = c0 - 32 * q4;  // first column i, and its place from the diagonal block
+            uint32_t pp[8], ee[8];
+            if (d0 < 0) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) pp[e] = ee[e] = 0;
+            } else {
+              float a2[16];
+              tc::tmem_ld16(tl + kColA2 + c0, a2);
+              float f[16];
+              if (d0 >= 32) {
+                const float bf = block_f[b >> 1];
+                const float4* rr = reinterpret_cast<const float4*>(sm.r + c0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float4 x = rr[e];
+                  f[4 * e] = x.x * bf; f[4 * e + 1] = x.y * bf; f[4 * e + 2] = x.z * bf; f[4 * e + 3] = x.w * bf;
+                }
+              } else {
+                const float4* gg = reinterpret_cast<const float4*>(sm.g2 + c0);
+                const int first = lane - d0;  // columns from this one on are not in the past
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float4 x = gg[e];
+                  const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                  for (int u = 0; u < 4; ++u) f[4 * e + u] = 4 * e + u >= first ? p.a.scale * exp2_approx(y[u] - gj) : 0.f;
+                }
+              }
+              tc::tmem_wait_ld();
+              const int first = d0 >= 32 ? 0 : lane - d0;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {  // (a select: what lies in the past may not be finite)
+                a1[b][e] = e >= first ? a1[b][e] * f[e] : 0.f;
+                a2[e] = e >= first ? a2[e] * f[e] : 0.f;
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                pp[e] = pack_bf16(a1[b][2 * e], a1[b][2 * e + 1]);
+                ee[e] = pack_bf16(a2[2 * e], a2[2 * e + 1]);
+              }
+            }
+            tc::tmem_st8(tl + kColA1 + 64 * half + 8 * b, pp);
+            tc::tmem_st8(tl + kColA1 + 64 * half + 32 + 8 * b, ee);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<uint4*>(erow + (((2 * b + e) ^ (row & 7)) << 4)) =
+                  make_uint4(ee[4 * e], ee[4 * e + 1], ee[4 * e + 2], ee[4 * e + 3]);
+          }
+          tc::tmem_wait_st();
+          tc::fence_proxy_async();
+          tc::tc_fence_before();
+          tc::mbar_arrive(&sm.pe);
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sm.f_empty);
+        }
+        // ---- the products with the states: row factors ----------------------
+        if (!(ok = warp_wait(&sm.g2_, par))) break;
+        tc::tc_fence_after();
+        float kin = 0.f, sdot = 0.f;
+        const unsigned char* krow = tile(kTK) + (K == 128 ? half * kTile : 0) + row * 128;
+        const unsigned char* qrow = tile(kTQ) + (K == 128 ? half * kTile : 0) + row * 128;
+        constexpr int kTurns = K / 32;  // of 16 columns, per half
+        const int p0 = K == 128 ? 0 : 4 * half;  // first 16-byte piece of this half's columns in the row
+        const uint64_t of2 = tc::pack2(out_f, out_f), if2 = tc::pack2(in_f, in_f);
+#pragma unroll 1
+        for (int b = 0; b < kTurns; ++b) {
+          float x[16], y[16];
+          const uint32_t cq = tl + kColDq + half * (K / 2) + 16 * b, ck = tl + kColDk + half * (K / 2) + 16 * b;
+          tc::tmem_ld16(cq, x);
+          tc::tmem_ld16(ck, y);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            tc::unpack2(tc::mul2(tc::pack2(x[e], x[e + 1]), of2), x[e], x[e + 1]);
+            tc::unpack2(tc::mul2(tc::pack2(y[e], y[e + 1]), if2), y[e], y[e + 1]);
+          }
+          tc::tmem_st16f(cq, x);
+          tc::tmem_st16f(ck, y);
+          if constexpr (kDg) kin += dot16(krow, p0 + 2 * b, row, y);
+        }
+        if constexpr (kDg) {  // <S, dS'>: this thread's share of the tiles
+          const uint4* s4 = reinterpret_cast<const uint4*>(tile(kTS));
+          const uint4* d4 = reinterpret_cast<const uint4*>(tile(kTD));
+#pragma unroll 2
+          for (int e = tid - 128; e < K * V / 8; e += 256) sdot += dot8(s4[e], d4[e]);
+          sdot *= eGC;
+        }
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        tc::mbar_arrive(&sm.rmw1);
+        release(kTS);
+        release(kTD);
+        release(kTV);
+        release(kTO);
+        if (!(ok = warp_wait(&sm.g3, par))) break;
+        tc::tc_fence_after();
+#pragma unroll 1
+        for (int b = 0; b < V / 32; ++b) {
+          float x[16];
+          const uint32_t cv = tl + kColA2 + half * (V / 2) + 16 * b;
+          tc::tmem_ld16(cv, x);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) tc::unpack2(tc::mul2(tc::pack2(x[e], x[e + 1]), if2), x[e], x[e + 1]);
+          tc::tmem_st16f(cv, x);
+        }
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        tc::mbar_arrive(&sm.rmw2);
+        // ---- results ---------------------------------------------------------
+        if (!(ok = warp_wait(&sm.g4a, par))) break;
+        tc::tc_fence_after();
+        float xy = 0.f;
+#pragma unroll 1
+        for (int z = 0; z < 2; ++z) {  // dq, dk
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(z ? p.gr.dk : p.gr.dq) + (tok * H + w.h) * K + half * (K / 2);
+          float* sum = acc + (int64_t)z * kC * K;
+#pragma unroll 1
+          for (int b = 0; b < kTurns; ++b) {
+            float x[16];
+            tc::tmem_ld16(tl + (z ? kColDk : kColDq) + half * (K / 2) + 16 * b, x);
+            tc::tmem_wait_ld();
+            if constexpr (kDg) {
+              const float d = dot16(z ? krow : qrow, p0 + 2 * b, row, x);
+              xy += z ? -d : d;
+            }
+            if (group > 1) {  // this CTA's running sums over the value heads of the group
+              if (j > 0) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                  const float4 y = *reinterpret_cast<const float4*>(sum + 16 * b + e);
+                  x[e] += y.x; x[e + 1] += y.y; x[e + 2] += y.z; x[e + 3] += y.w;
+                }
+              }
+              if (j + 1 < group) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                  *reinterpret_cast<float4*>(sum + 16 * b + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+              }
+            }
+            if (inside && j + 1 == group) st_32bytes(out + 16 * b, pack8(x), pack8(x + 8));
+          }
+          release(z ? kTK : kTQ);
+        }
+        tc::tc_fence_before();
+        tc::mbar_arrive(&sm.qk_free);
+        if (!(ok = warp_wait(&sm.g4b, par))) break;
+        tc::tc_fence_after();
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.gr.dv) + (tok * HV + hv) * V + half * (V / 2);
+#pragma unroll 1
+        for (int b = 0; b < V / 32; ++b) {
+          float x[16];
+          tc::tmem_ld16(tl + kColA2 + half * (V / 2) + 16 * b, x);
+          tc::tmem_wait_ld();
+          if (inside) st_32bytes(out + 16 * b, pack8(x), pack8(x + 8));
+        }
+        tc::tc_fence_before();
+        tc::mbar_arrive(&sm.dv_free);
+        if constexpr (kDg) {
+          if (n > 0 && !(ok = warp_wait(&sm.xy_free, (n - 1) & 1))) break;
+          sm.xy[half][row] = xy;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            kin += __shfl_xor_sync(0xffffffffu, kin, o);
+            sdot += __shfl_xor_sync(0xffffffffu, sdot, o);
+          }
+          if (lane == 0) {
+            sm.part[warp - 4] = kin;
+            sm.part[warp + 4] = sdot;
+          }
+          tc::mbar_arrive(&sm.xy_full);
+        }
+      }
+    }
+  }
+  if (!ok) atomicOr(&g_la_fault, 1u);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == 1) tc::tmem_dealloc(tb, 512);
+}
+
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
@@ -688,6 +1238,15 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
       fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   }
   return fn;
+}
+
+// The driver call above needs the device's context to be current.  A thread
+// whose first CUDA work is this call (autograd's, say) has none bound yet.
+int bind_context() {
+  int dev = 0;
+  GDN2_CUDA_TRY(cudaGetDevice(&dev));
+  GDN2_CUDA_TRY(cudaSetDevice(dev));
+  return 0;
 }
 
 // [B, T, H, D] bf16 with the given element steps -> boxes of 128 tokens x 64
@@ -764,6 +1323,7 @@ int la_tc_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_
   p.tasks = p.seg.entries * a.HV * (a.V / 64);
   if (p.tasks >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
   const bool save = a.flags & GDN2_SAVE_FOR_BWD;
+  if (int st = bind_context()) return st;
   ScanMaps m;
   if (!token_map(&m.x, a.k, a.K, a.H, a.T, a.B, a.k_stride) || !token_map(&m.q, a.q, a.K, a.H, a.T, a.B, a.q_stride) ||
       !token_map(&m.y, a.v, a.V, a.HV, a.T, a.B, a.v_stride))
@@ -772,6 +1332,52 @@ int la_tc_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_
   if (save && !state_map(&m.s, ws.states16, a.V, la_num_chunks(a) * a.HV * a.K, a.K)) return GDN2_ERR_TENSOR_MAP;
   const bool exact = a.flags & GDN2_STORE_FINAL;
   return a.K == 128 ? scan<128, false>(p, m, true, save, exact, s) : scan<64, false>(p, m, true, save, exact, s);
+}
+
+namespace {
+
+template <int K, int V, bool kDg>
+int run_bwd(const BwdArgs& p, const CUtensorMap (&m)[6], cudaStream_t s) {
+  auto kern = la_bwd_tc_kernel<K, V, kDg>;
+  static_assert(sizeof(BwdSmem) <= 227 * 1024, "shared memory of the backward");
+  GDN2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BwdSmem)));
+  ProfScope ps(kKLinAttnBwd, s);
+  kern<<<(unsigned)std::min<int64_t>(p.items, kLaSms), 384, sizeof(BwdSmem), s>>>(p, m[0], m[1], m[2], m[3], m[4], m[5]);
+  GDN2_LAUNCH_CHECK();
+  return 0;
+}
+
+template <int K, int V>
+int bwd(const BwdArgs& p, const CUtensorMap (&m)[6], cudaStream_t s) {
+  return p.gr.dg ? run_bwd<K, V, true>(p, m, s) : run_bwd<K, V, false>(p, m, s);
+}
+
+}  // namespace
+
+int la_tc_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
+                     const LaBwdWs& bw, cudaStream_t s) {
+  ScanArgs sc{a, la_decay(a), la_geom(a, ws), la_segs(a, bw.seg), 0, 0, gr.dht, gr.dh0};
+  if (sc.seg.cut) {  // the forward's map of the cut
+    sc.seg.map = ws.seg.map;
+    sc.seg.first = ws.seg.first;
+  }
+  sc.tasks = sc.seg.entries * a.HV * (a.V / 64);
+  BwdArgs p{a, gr, la_decay(a), la_geom(a, ws), la_num_chunks(a) * a.H, bw.acc, a.decay == GDN2_DECAY_HEAD ? bw.dg : nullptr};
+  if (sc.tasks >= (int64_t(1) << 31) || p.items >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
+  const int64_t ostep[3] = {a.T * a.HV * a.V, a.HV * a.V, a.V}, rows = la_num_chunks(a) * a.HV * a.K;
+  if (int st = bind_context()) return st;
+  CUtensorMap m[6];  // q, k, v, do, S, dS'
+  if (!token_map(&m[0], a.q, a.K, a.H, a.T, a.B, a.q_stride) || !token_map(&m[1], a.k, a.K, a.H, a.T, a.B, a.k_stride) ||
+      !token_map(&m[2], a.v, a.V, a.HV, a.T, a.B, a.v_stride) ||
+      !token_map(&m[3], gr.dout, a.V, a.HV, a.T, a.B, ostep) || !state_map(&m[4], ws.states16, a.V, rows, a.K) ||
+      !state_map(&m[5], bw.dstates16, a.V, rows, a.K))
+    return GDN2_ERR_TENSOR_MAP;
+  const ScanMaps sm{m[0], m[0], m[3], m[5]};
+  const bool exact = gr.dh0 != nullptr;
+  if (int st = a.K == 128 ? scan<128, true>(sc, sm, false, true, exact, s) : scan<64, true>(sc, sm, false, true, exact, s))
+    return st;
+  if (a.K == 128) return a.V == 128 ? bwd<128, 128>(p, m, s) : bwd<128, 64>(p, m, s);
+  return a.V == 128 ? bwd<64, 128>(p, m, s) : bwd<64, 64>(p, m, s);
 }
 
 int la_fault_read(int clear, unsigned int* out) {

@@ -19,7 +19,7 @@ const char* kNames[kNumKernels] = {"chunk_intra_kernel", "chunk_scan_fwd_kernel"
                                    "norm_gate_fwd_kernel", "norm_gate_bwd_kernel", "seg_fold_kernel",
                                    "chunk_bwd_fp32_kernel", "fp32_prep_epilogue_kernel",
                                    "linear_attn_fp32_kernels", "linear_attn_recurrent_kernel", "linear_attn_scan_kernel",
-                                   "linear_attn_states_kernel",
+                                   "linear_attn_states_kernel", "linear_attn_bwd_kernel",
                                    "layer_norm_fwd_kernel", "layer_norm_bwd_kernel"};
 
 struct Pending {

@@ -249,6 +249,17 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&x)[16]) {
   for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ void tmem_st16f(uint32_t taddr, const float (&x)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(__float_as_uint(x[0])), "r"(__float_as_uint(x[1])), "r"(__float_as_uint(x[2])), "r"(__float_as_uint(x[3])),
+      "r"(__float_as_uint(x[4])), "r"(__float_as_uint(x[5])), "r"(__float_as_uint(x[6])), "r"(__float_as_uint(x[7])),
+      "r"(__float_as_uint(x[8])), "r"(__float_as_uint(x[9])), "r"(__float_as_uint(x[10])), "r"(__float_as_uint(x[11])),
+      "r"(__float_as_uint(x[12])), "r"(__float_as_uint(x[13])), "r"(__float_as_uint(x[14])), "r"(__float_as_uint(x[15]))
+      : "memory");
+}
+
 // 8 consecutive 32-bit columns of this thread's lane (16 packed bf16: the
 // layout of a 16-bit A operand in TMEM, two elements of a row per column)
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&x)[8]) {

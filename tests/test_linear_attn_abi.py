@@ -35,8 +35,9 @@ def test_linear_attn_alignment_workspace_and_flags(gdn2):
     ptrs = dict(q=p, k=p, v=p, o=p)
     assert lib.gdn2_linear_attn_fwd(_la(gdn2, **{**ptrs, "q": p + 2}), None, 0, None) == 5
     assert lib.gdn2_linear_attn_fwd(_la(gdn2, **ptrs, v_stride=L._s3(51200, 516, 128)), None, 0, None) == 5
-    assert lib.gdn2_linear_attn_fwd(_la(gdn2, **ptrs), None, 0, None) == 6
-    assert lib.gdn2_linear_attn_workspace_size(_la(gdn2)) > 0
+    assert lib.gdn2_linear_attn_fwd(_la(gdn2, **ptrs, flags=L.SAVE_FOR_BWD), None, 0, None) == 6
+    assert lib.gdn2_linear_attn_workspace_size(_la(gdn2, flags=L.SAVE_FOR_BWD)) >= 2 * 1 * 4 * 64 * 128 * 2
+    assert lib.gdn2_linear_attn_workspace_size(_la(gdn2)) == 0  # one segment, nothing kept
     assert lib.gdn2_linear_attn_workspace_size(_la(gdn2, K=100)) == 0
     grads = L.LinearAttnGrads(dout=p, dq=p, dk=p, dv=p)
     assert lib.gdn2_linear_attn_bwd(_la(gdn2, **ptrs), grads, None, 0, None, 0, None) == 7  # no SAVE_FOR_BWD

@@ -9,7 +9,9 @@ Tolerances (relative 2-norm), from the roundings of each path:
   initial state's gradient of the bf16 path): sums of a few hundred terms in
   fp32, or of products whose operands carry 16 bits or more: below 1e-5.
 * the gradient of g is a difference of sums: its error is held against the
-  magnitude of the terms, not of the difference.
+  magnitude of the terms, not of the difference.  Each term carries three
+  roundings (the decayed scores and both states of a product), one rounding to
+  8 significant bits being 1.7e-3 in the rms: together 2.9e-3, and twice that.
 """
 
 import itertools
@@ -116,7 +118,7 @@ def check(got, want, d, dtype, names=("o", "ht", "dq", "dk", "dv", "dg", "dh0", 
             err = (got[n].detach().double().cpu() - want[n]).norm() / want[n].numel() ** 0.5
             ref = want[n].norm() / want[n].numel() ** 0.5
             scale = max(float(ref), dg_mass(d, want) * (1.0 if d["g"].ndim == 3 else want["dq"].shape[1] ** 0.5))
-            t = TOL[torch.bfloat16 if dtype == torch.bfloat16 else torch.float32]
+            t = 6e-3 if dtype == torch.bfloat16 else TOL[dtype]
             assert float(err) <= t * scale, f"dg: {float(err):.3e} of {scale:.3e}"
         else:
             assert rel(got[n], want[n]) <= tol, f"{n}: {rel(got[n], want[n]):.3e} > {tol}"
