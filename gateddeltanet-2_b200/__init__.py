@@ -32,8 +32,8 @@ import sys as _sys
 from . import _lib, cp
 from .chunk import ChunkGDN2Function, chunk_gdn2, gdn2_telemetry_snapshot, prepare_chunk_indices
 from .layer import FusedRMSNormSwishGate, GatedDeltaNet2, LayerCache, ShortConvolution
-from .layer_norm import LayerNorm, LayerNormFunction, layer_norm
-from .linear_attn import ChunkLinearAttnFunction, chunk_linear_attn, fused_recurrent_linear_attn
+from .layer_norm import LayerNorm, layer_norm
+from .linear_attn import chunk_linear_attn, fused_recurrent_linear_attn
 from .linear_layer import LinearAttention
 from .recurrent import fused_recurrent_gdn2, fused_recurrent_gdn2_fwd
 
@@ -52,10 +52,8 @@ __all__ = [
     "ShortConvolution",
     "FusedRMSNormSwishGate",
     "chunk_linear_attn",
-    "ChunkLinearAttnFunction",
     "fused_recurrent_linear_attn",
     "layer_norm",
     "LayerNorm",
-    "LayerNormFunction",
     "LinearAttention",
 ]

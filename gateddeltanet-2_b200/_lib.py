@@ -90,14 +90,13 @@ class PrepGrads(ctypes.Structure):
     ]
 
 
-_s3 = _i64 * 3
-
-
 class LinearAttnArgs(ctypes.Structure):
     _fields_ = [
         ("B", _i64), ("T", _i64), ("H", _i64), ("HV", _i64), ("K", _i64), ("V", _i64),
         ("N", _i64),
-        ("q_stride", _s3), ("k_stride", _s3), ("v_stride", _s3), ("g_stride", _s3),
+        # element steps of batch, token and head (int64[3] each in the header)
+        ("q_b", _i64), ("q_t", _i64), ("q_h", _i64), ("k_b", _i64), ("k_t", _i64), ("k_h", _i64),
+        ("v_b", _i64), ("v_t", _i64), ("v_h", _i64), ("g_b", _i64), ("g_t", _i64), ("g_h", _i64),
         ("cu_seqlens", _p), ("state_indices", _p), ("num_slots", _i64),
         ("state_stride_in", _i64), ("state_stride_out", _i64),
         ("scale", _f32), ("flags", _i32), ("dtype", _i32), ("dtype_g", _i32), ("decay", _i32),
@@ -239,25 +238,32 @@ def ptr(t) -> int | None:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    idx = device.index
+    # (the raw handle: a tenth of the cost of building the stream object around it)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
-class on_device:
-    """``torch.cuda.device`` without its cost where the device is current already."""
+_ops = None
+OPS_PATH = os.path.join(_HERE, "_torch_ops.so")
 
-    __slots__ = ("guard",)
 
-    def __init__(self, device: torch.device):
-        here = device.index is None or device.index == torch.cuda.current_device()
-        self.guard = None if here else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def ops():
+    """The torch functions of csrc/torch_ops.cpp (linear attention, layer norm), bound to the loaded library."""
+    global _ops
+    if _ops is None:
+        if not os.path.exists(OPS_PATH):
+            raise ImportError(f"{OPS_PATH} is missing: build it with `python gateddeltanet-2_b200/build.py`")
+        from importlib import machinery, util
+        spec = util.spec_from_loader("_torch_ops", machinery.ExtensionFileLoader("_torch_ops", OPS_PATH))
+        mod = util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        lib = load()
+        mod.init([ctypes.cast(getattr(lib, "gdn2_" + n), _p).value for n in (
+            "linear_attn_workspace_size", "linear_attn_fwd", "linear_attn_bwd_workspace_size", "linear_attn_bwd",
+            "linear_attn_recurrent_fwd", "layer_norm_fwd", "layer_norm_bwd_workspace_size", "layer_norm_bwd",
+            "status_string", "device_supported")])
+        _ops = mod
+    return _ops
 
 
 _checked_devices: set[int] = set()

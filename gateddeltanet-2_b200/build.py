@@ -1,4 +1,5 @@
-"""Build libgdn2_b200.so (all CUDA sources, sm_100a) next to this file.
+"""Build libgdn2_b200.so (all CUDA sources, sm_100a) and _torch_ops.so (its
+torch functions, against the installed torch) next to this file.
 
 ``python gateddeltanet-2_b200/build.py`` or ``build()`` from Python.  Objects
 go to ``_build/`` at the repository root; a source is recompiled when it or
@@ -51,8 +52,38 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_ops(verbose: bool) -> str:
+    src, out = os.path.join(CSRC, "torch_ops.cpp"), os.path.join(PKG_DIR, "_torch_ops.so")
+    if os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), _newest_header()):
+        return out
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"], INCLUDE]
+    libs = ["c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python"]
+    cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *("-I" + i for i in inc), src, "-o", out, "-L" + os.path.join(root, "lib"), *("-l" + x for x in libs)]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src}:\n{r.stdout}\n{r.stderr}")
+    return out
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD_DIR, exist_ok=True)
+    with cf.ThreadPoolExecutor(max_workers=1) as ex:
+        ops = ex.submit(_build_ops, verbose)
+        lib = _build_lib(verbose)
+        ops.result()
+    return lib
+
+
+def _build_lib(verbose: bool) -> str:
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))

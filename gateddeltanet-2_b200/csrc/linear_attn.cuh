@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 
@@ -10,6 +11,19 @@ namespace gdn2 {
 
 constexpr int kLaChunkF32 = 64;   // tokens per chunk of the fp32 kernels
 constexpr int kLaChunkTc = 128;   // and of the tensor-core kernels
+// The shared-memory opt-in of a kernel, asked for once per device.
+template <auto kKernel>
+inline int smem_opt_in(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  GDN2_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  GDN2_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
+
 constexpr int kLaSms = 148;       // CTAs of a persistent kernel: one per SM of a B200
 
 // A chunk of a packed batch: its sequence (-1: past the last chunk) and its index there.

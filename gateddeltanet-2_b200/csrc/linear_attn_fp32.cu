@@ -544,12 +544,6 @@ __global__ void __launch_bounds__(256) la_zero_outside_kernel(LaRows r, LaGeom g
   }
 }
 
-template <typename F>
-int set_smem(F f, size_t bytes) {
-  GDN2_CUDA_TRY(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  return 0;
-}
-
 template <typename T, int K, int V>
 int fwd(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
   const LaGeom geo = la_geom(a, ws);
@@ -561,7 +555,7 @@ int fwd(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
   ProfScope ps(kKLinAttnFp32, s);
   if (NT > 0) {
     const size_t sm = kC * (K + 1 + V + 1) * 4;
-    if (int st = set_smem(la_state_kernel<T, K, V, false>, sm)) return st;
+    if (int st = (smem_opt_in<la_state_kernel<T, K, V, false>>(sm))) return st;
     la_state_kernel<T, K, V, false><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
         static_cast<const T*>(a.k), a.k_stride[0], a.k_stride[1], a.k_stride[2], static_cast<const T*>(a.v),
         a.v_stride[0], a.v_stride[1], a.v_stride[2], dec, geo, HV, group, 1.f, ws.states, ws.total);
@@ -572,7 +566,7 @@ int fwd(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
   GDN2_LAUNCH_CHECK();
   if (NT > 0) {
     const size_t sm = (2 * kC * (K + 1) + kC * (V + 1) + kC * kLdP + 64 * (V + 1)) * 4;
-    if (int st = set_smem(la_out_kernel<T, K, V>, sm)) return st;
+    if (int st = (smem_opt_in<la_out_kernel<T, K, V>>(sm))) return st;
     la_out_kernel<T, K, V><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(a, dec, geo, ws.states);
     GDN2_LAUNCH_CHECK();
   }
@@ -589,7 +583,7 @@ int bwd(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const 
   ProfScope ps(kKLinAttnFp32, s);
   if (NT > 0) {
     const size_t sm = kC * (K + 1 + V + 1) * 4;
-    if (int st = set_smem(la_state_kernel<T, K, V, true>, sm)) return st;
+    if (int st = (smem_opt_in<la_state_kernel<T, K, V, true>>(sm))) return st;
     la_state_kernel<T, K, V, true><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
         static_cast<const T*>(a.q), a.q_stride[0], a.q_stride[1], a.q_stride[2], static_cast<const T*>(gr.dout),
         a.T * HV * V, (int64_t)HV * V, V, dec, geo, HV, group, a.scale, bw.dstates, nullptr);
@@ -601,7 +595,7 @@ int bwd(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const 
   if (NT > 0) {
     constexpr int half = 64 * (V + 1) > K * 65 ? 64 * (V + 1) : K * 65;
     const size_t sm = (2 * kC * (K + 1) + 2 * kC * (V + 1) + 2 * kC * kLdP + half) * 4;
-    if (int st = set_smem(la_bwd_kernel<T, K, V>, sm)) return st;
+    if (int st = (smem_opt_in<la_bwd_kernel<T, K, V>>(sm))) return st;
     la_bwd_kernel<T, K, V><<<dim3((unsigned)NT, (unsigned)a.H), kThreads, sm, s>>>(
         a, gr, dec, geo, ws.states, bw.dstates, a.decay == GDN2_DECAY_HEAD ? bw.dg : nullptr);
     GDN2_LAUNCH_CHECK();

@@ -19,17 +19,15 @@
 //               e^{G_i - G_r} e^{G_r - G_j} with r the first row of the 32-row block:
 //               both factors are at most 1 for decays, one is per row, the other per
 //               block and column, so only the 32 diagonal columns take an exponential each.
-//   warps 12-15 half of w v in bf16, and the state in registers (thread = row k of
-//               S): S <- e^{G_C} S + what the MMA left in TMEM; bf16 copy for Q S
-//   warps 16-19 the other half of w v; o out of TMEM (thread = token), straight to
-//               memory, 32 bytes a store
+//   warps 12-15 the state in registers (thread = row k of S): S <- e^{G_C} S + what
+//               the MMA left in TMEM; bf16 copy for Q S (without outputs also w v)
+//   warps 16-19 w v; o out of TMEM (thread = token), straight to memory, 32 bytes a store
 // MMA order per chunk i: Q K^T, K^T (w v), then P V of chunk i - 1, then Q S.  The
 // lag gives the scores more than a chunk's time, and a q, k stage is held only
 // from its first product to its last, so two stages cover the loads' latency.
-// Precision: P, S, w and w v are rounded to bf16 for the MMAs (as the result
-// itself is).  Where the final state (or the initial state's gradient) is
-// asked for, w v goes in as the sum of two bf16 values, so the state that leaves
-// in fp32 carries 16 bits or more of every product.
+// Precision: P and S are rounded to bf16 as MMA operands (as the result itself
+// is).  w v goes in as the sum of two bf16 values, so the fp32 state carries 16
+// bits or more of every product: with one it would hold 8, and o as many again less.
 // Every wait is bounded (tc::kWaitLimitNs); one that gives up sets g_la_fault.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -64,18 +62,18 @@ GDN2_DEV float sum_diff(const Sums& g, int i, int j) {
   return (g.hi[i] - g.hi[j]) + (__bfloat162float(g.lo[i]) - __bfloat162float(g.lo[j]));
 }
 
-template <int K, bool kOut, bool kExact>
+template <int K, bool kOut>
 struct alignas(1024) ScanSmem {
   static constexpr int NX = kOut ? 2 : 3, NY = 3;  // stages
   static constexpr int NB = kOut ? 1 : 2;          // chunks of w v held
   __nv_bfloat16 X[NX][(kOut ? 2 : 1) * K / 64][128 * 64];  // k; with outputs then q
   __nv_bfloat16 Y[NY][128 * 64];
-  __nv_bfloat16 YW[NB][kExact ? 2 : 1][128 * 64];
+  __nv_bfloat16 YW[NB][2][128 * 64];  // w v as the sum of two bf16 values
   __nv_bfloat16 S[K * 64];  // bf16 state, rows k
   Sums f[2];
   float cw[kOut ? 320 : 4];  // column factors of the score warps, 32 (w + 1) for w = 0..3
   uint64_t full_x[NX], empty_x[NX], full_y[NY], empty_y[NY], f_full[2], f_empty[2], qk_full[2], p_full[2];
-  uint64_t yw_full[NB], ds_full[NB], s_full, s_free, o_full, o_free, aborted;
+  uint64_t yw_full[NB], ds_full[NB], ds_free, s_full, s_free, o_full, o_free, aborted;
   uint32_t tbase;
 };
 
@@ -176,12 +174,12 @@ GDN2_DEV bool warp_wait(uint64_t* bar, uint32_t parity) {
   return r;
 }
 
-template <int K, bool kOut, bool kStore, bool kBack, bool kExact>
+template <int K, bool kOut, bool kStore, bool kBack>
 __global__ void __launch_bounds__(kOut ? 640 : 256, 1)
 la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmQ,
                const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmS) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  using Sm = ScanSmem<K, kOut, kExact>;
+  using Sm = ScanSmem<K, kOut>;
   Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
   constexpr uint32_t NX = Sm::NX, NY = Sm::NY, NB = Sm::NB;
   // TMEM columns: two score buffers, Q S of two chunks, P V, the state term
@@ -199,14 +197,15 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sm.f_full[i], 32);
-      tc::mbar_init(&sm.f_empty[i], kOut ? 16 : 4);
+      tc::mbar_init(&sm.f_empty[i], kOut ? 16 : 4);  // one per warp that reads them
       tc::mbar_init(&sm.qk_full[i], 1);
       tc::mbar_init(&sm.p_full[i], 256);
     }
     for (uint32_t i = 0; i < NB; ++i) {
-      tc::mbar_init(&sm.yw_full[i], kOut ? 256 : 128);
+      tc::mbar_init(&sm.yw_full[i], 128);
       tc::mbar_init(&sm.ds_full[i], 1);
     }
+    tc::mbar_init(&sm.ds_free, 128);
     tc::mbar_init(&sm.s_full, 128);
     tc::mbar_init(&sm.s_free, 1);
     tc::mbar_init(&sm.o_full, 1);
@@ -227,68 +226,69 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
   // the token coordinate and batch of chunk c in the tensor maps
   auto tok = [&](int c) { return (int)((p.geo.cu ? t.bos : 0) + (int64_t)c * kC); };
   const int64_t step = gridDim.x;
-  // w v of chunk `it`, 16-byte pieces q0 .. q0 + nq of this thread's token j.  Returns the chunk's sums it
-  // was made from through f_row (e^{G_j}) and total (e^{G_C}).
-  auto weigh = [&](int c, int j, auto q0, auto nq, float& f_row, float& total) -> bool {
-    const int s = it & 1, L = rows(c);
-    const uint32_t sy = it % NY, b = it % NB;
+  // w v of chunk `it`, row j of its tile (token j): made in registers, so that it can
+  // be ready before the MMAs have read the chunk before's, then put in shared memory.
+  // f_row: e^{G_j}, total: e^{G_C}.
+  uint32_t wh[32], wl[32];
+  auto prepare = [&](int c, int j, float& f_row, float& total) -> bool {
+    const int s = it & 1;
+    const uint32_t sy = it % NY;
     if (!warp_wait(&sm.f_full[s], (it >> 1) & 1)) return false;
     const Sums& g = sm.f[s];
-    const float hi_j = g.hi[j], last = g.hi[kC - 1] + __bfloat162float(g.lo[kC - 1]);
-    f_row = exp_of(hi_j);
-    total = exp_of(last);
-    const float f = j >= L ? 0.f : kBack ? p.a.scale * f_row : exp_of(sum_diff(g, kC - 1, j));
+    f_row = exp_of(g.hi[j]);
+    total = exp_of(g.hi[kC - 1] + __bfloat162float(g.lo[kC - 1]));
+    const float f = j >= rows(c) ? 0.f : kBack ? p.a.scale * f_row : exp_of(sum_diff(g, kC - 1, j));
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(&sm.f_empty[s]);
     const uint32_t fh = pack_bf16(f, f);
     const float fr = f - bf16_round(f);
     const uint32_t fl = pack_bf16(fr, fr);
-    char* src = reinterpret_cast<char*>(sm.Y[sy]) + j * 128;
-    char* hi = reinterpret_cast<char*>(sm.YW[b][0]) + j * 128;
-    [[maybe_unused]] char* lo = reinterpret_cast<char*>(sm.YW[b][kExact ? 1 : 0]) + j * 128;
+    const char* src = reinterpret_cast<const char*>(sm.Y[sy]) + j * 128;
     if (!warp_wait(&sm.full_y[sy], (it / NY) & 1)) return false;
-    if (NB == 1 && it > 0 && !warp_wait(&sm.ds_full[0], (it - 1) & 1)) return false;  // YW has been read
-#pragma unroll 4
-    for (int q = q0; q < q0 + nq; ++q) {
-      const int at = (q ^ (j & 7)) << 4;
-      const uint4 v4 = *reinterpret_cast<const uint4*>(src + at);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const uint4 v4 = *reinterpret_cast<const uint4*>(src + ((q ^ (j & 7)) << 4));
       const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
-      uint32_t h[4];
-      [[maybe_unused]] uint32_t l[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        h[e] = tc::bmul2(v[e], fh);
+        const uint32_t h = tc::bmul2(v[e], fh);
         // what the product of the leading parts lost (exact), and the trailing part's product
-        if constexpr (kExact) l[e] = tc::bfma2(v[e], fl, tc::bfma2(v[e], fh, h[e] ^ 0x80008000u));
+        wl[4 * q + e] = tc::bfma2(v[e], fl, tc::bfma2(v[e], fh, h ^ 0x80008000u));
+        wh[4 * q + e] = h;
       }
-      *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-      if constexpr (kExact) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
     }
-    if (p.geo.cu && L < kC) {  // the next sequence's rows in this tile: none of them may reach a sum
-      if (!warp_wait(&sm.full_x[it % NX], (it / NX) & 1)) return false;
-      if (j >= L) {
-#pragma unroll 1
-        for (int q = q0; q < q0 + nq; ++q) {
-          const int at = (q ^ (j & 7)) << 4;
-          *reinterpret_cast<uint4*>(src + at) = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(hi + at) = make_uint4(0, 0, 0, 0);
-          if constexpr (kExact) *reinterpret_cast<uint4*>(lo + at) = make_uint4(0, 0, 0, 0);
+    return true;
+  };
+  auto put = [&](int c, int j) -> bool {
+    const uint32_t sy = it % NY, b = it % NB;
+    const int L = rows(c);
+    char* hi = reinterpret_cast<char*>(sm.YW[b][0]) + j * 128;
+    char* lo = reinterpret_cast<char*>(sm.YW[b][1]) + j * 128;
+    // rows of the next sequence in this tile: none of them may reach a sum
+    const bool clear = p.geo.cu && L < kC;
+    if (clear && !warp_wait(&sm.full_x[it % NX], (it / NX) & 1)) return false;
+    if (it >= NB && !warp_wait(&sm.ds_full[b], (it / NB - 1) & 1)) return false;  // YW has been read
+    if (clear && j >= L) {
 #pragma unroll
-          for (int e = 0; e < K / 64; ++e)
-            *reinterpret_cast<uint4*>(reinterpret_cast<char*>(sm.X[it % NX][e]) + j * 128 + at) = make_uint4(0, 0, 0, 0);
-        }
+      for (int q = 0; q < 32; ++q) wh[q] = wl[q] = 0;
+      for (int q = 0; q < 8; ++q) {
+        *reinterpret_cast<uint4*>(reinterpret_cast<char*>(sm.Y[sy]) + j * 128 + 16 * q) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < K / 64; ++e)
+          *reinterpret_cast<uint4*>(reinterpret_cast<char*>(sm.X[it % NX][e]) + j * 128 + 16 * q) = make_uint4(0, 0, 0, 0);
       }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int at = (q ^ (j & 7)) << 4;
+      *reinterpret_cast<uint4*>(hi + at) = make_uint4(wh[4 * q], wh[4 * q + 1], wh[4 * q + 2], wh[4 * q + 3]);
+      *reinterpret_cast<uint4*>(lo + at) = make_uint4(wl[4 * q], wl[4 * q + 1], wl[4 * q + 2], wl[4 * q + 3]);
     }
     tc::fence_proxy_async();
     tc::mbar_arrive(&sm.yw_full[b]);
     if constexpr (!kOut) tc::mbar_arrive(&sm.empty_y[sy]);
     return true;
   };
-  using std::integral_constant;
-  const integral_constant<int, 0> kQ0{};
-  const integral_constant<int, 4> kHalf{};
-  const integral_constant<int, 8> kAll{};
-
 
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
@@ -329,6 +329,13 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       constexpr uint32_t iQK = tc::idesc_bf16(128, 128, 0, 0), iNV = tc::idesc_bf16(128, 64, 0, 1);
       constexpr uint32_t iDS = tc::idesc_bf16(K, 64, 1, 1);
       const uint32_t aX = addr16(sm.X), aY = addr16(sm.Y), aW = addr16(sm.YW), aS = addr16(sm.S);
+      // MMAs of 16 along k, one after the other
+      auto mmas = [&](auto steps, auto issue) {
+#pragma unroll
+        for (int kk = 0; kk < steps; ++kk) issue(kk);
+      };
+      constexpr std::integral_constant<int, K / 16> kSteps{};
+      constexpr std::integral_constant<int, 8> tSteps{};  // over the tokens
       uint32_t total = 0;  // chunks over all tasks
       for (int64_t id = blockIdx.x; id < p.tasks; id += step)
         if (find_task<kBack>(p, id, t)) total += (uint32_t)max(t.ce - t.cb, 0);
@@ -339,20 +346,21 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
           if (!(ok = wait(&sm.full_x[sx], (it / NX) & 1))) break;
           if constexpr (kOut) {
             tc::tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < K / 16; ++kk)
-              tc::mma_bf16(tb + kColQK + 128 * s, kmaj(aq, kk), kmaj(ax, kk), iQK,
-                           kk > 0);
+            mmas(kSteps, [&](int kk) {
+              tc::mma_bf16(tb + kColQK + 128 * s, kmaj(aq, kk), kmaj(ax, kk), iQK, kk > 0);
+            });
             tc::mma_commit(&sm.qk_full[s]);
           }
           if (!(ok = wait(&sm.yw_full[b], (it / NB) & 1))) break;
+          if constexpr (kOut) {  // the state term of the chunk before has left TMEM
+            if (it > 0 && !(ok = wait(&sm.ds_free, (it - 1) & 1))) break;
+          }
           tc::tc_fence_after();
 #pragma unroll
-          for (int e = 0; e < (kExact ? 2 : 1); ++e)
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              tc::mma_bf16(tb + kColDS + 64 * b, nmaj(ax, kk),
-                                nmaj(aW + (b * (kExact ? 2 : 1) + e) * (kTile >> 4), kk), iDS, e + kk > 0);
+          for (int e = 0; e < 2; ++e)
+            mmas(tSteps, [&](int kk) {
+              tc::mma_bf16(tb + kColDS + 64 * b, nmaj(ax, kk), nmaj(aW + (2 * b + e) * (kTile >> 4), kk), iDS, e + kk > 0);
+            });
           tc::mma_commit(&sm.ds_full[b]);
           if constexpr (!kOut) tc::mma_commit(&sm.empty_x[sx]);
         }
@@ -363,19 +371,19 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
             const uint32_t j = it - 1, sj = j & 1, sy = j % NY;
             if (!(ok = wait(&sm.full_y[sy], (j / NY) & 1) && wait(&sm.p_full[sj], (j >> 1) & 1))) break;
             tc::tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)  // P: columns 0-31 and 64-95 of the score buffer
-              tc::mma_bf16_ts(tb + kColO2, tb + kColQK + 128 * sj + 8 * kk + (kk < 4 ? 0 : 32), nmaj(aY + sy * (kTile >> 4), kk), iNV,
-                              kk > 0);
+            mmas(tSteps, [&](int kk) {  // P: columns 0-31 and 64-95 of the score buffer
+              tc::mma_bf16_ts(tb + kColO2, tb + kColQK + 128 * sj + 8 * kk + (kk < 4 ? 0 : 32),
+                              nmaj(aY + sy * (kTile >> 4), kk), iNV, kk > 0);
+            });
             tc::mma_commit(&sm.o_full);
             tc::mma_commit(&sm.empty_y[sy]);
           }
           if (it < total) {
             if (!(ok = wait(&sm.s_full, it & 1))) break;
             tc::tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < K / 16; ++kk)
+            mmas(kSteps, [&](int kk) {
               tc::mma_bf16(tb + kColO1 + 64 * s, kmaj(aq, kk), nmaj(aS, kk), iNV, kk > 0);
+            });
             tc::mma_commit(&sm.empty_x[sx]);  // also: S has been read
           }
         }
@@ -540,6 +548,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
         }
       }
       tc::tc_fence_before();
+      if constexpr (kOut) tc::mbar_arrive(&sm.ds_free);
       return true;
     };
     // the bf16 state of chunk `it`
@@ -570,16 +579,20 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
         st[4 * q] = x.x; st[4 * q + 1] = x.y; st[4 * q + 2] = x.z; st[4 * q + 3] = x.w;
       }
       const int nloc = t.ce - t.cb;
-      float unused;
       for (int i = 0; i <= nloc; ++i) {
-        if constexpr (NB == 2) {  // two buffers: w v before the MMA of the chunk before has ended
-          if (i < nloc && !(ok = weigh(nth(i), j, kQ0, kAll, unused, total_next))) break;
+        if constexpr (kOut) {
+          if (i < nloc) {
+            const int f = it & 1;
+            if (!(ok = warp_wait(&sm.f_full[f], (it >> 1) & 1))) break;
+            total_next = exp_of(sm.f[f].hi[kC - 1] + __bfloat162float(sm.f[f].lo[kC - 1]));
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sm.f_empty[f]);
+          }
+        } else {  // (two buffers: the next w v goes in before the MMA of the chunk before has ended)
+          float f_row;
+          if (i < nloc && !(ok = prepare(nth(i), j, f_row, total_next) && put(nth(i), j))) break;
         }
-        // (one buffer: the state term leaves TMEM before this half of w v lets the next one in)
         if (i > 0 && !(ok = take(it - 1))) break;
-        if constexpr (NB == 1) {
-          if (i < nloc && !(ok = weigh(nth(i), j, kQ0, kHalf, unused, total_next))) break;
-        }
         total = total_next;
         if (i == nloc) break;
         if constexpr (kOut || kStore) {
@@ -597,15 +610,15 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       }
     }
   } else if (kOut) {
-    // ------------------------------------------------------- output, half of w v
-    // Chunk it's half of w v comes before chunk it - 2's output, across tasks
-    // too: the MMAs of chunk it wait for the one and go before the other's end.
+    // ---------------------------------------------------------- w v, output
+    // Chunk it's w v comes before chunk it - 2's output, across tasks too: the
+    // MMAs of chunk it wait for the one and go before the other's end.
     const int w = warp & 3, i = 32 * w + lane;
     const uint32_t to = tb + ((uint32_t)(32 * w) << 16);
     const uint64_t sc2 = tc::pack2(p.a.scale, p.a.scale);
     const int64_t chunk_step = (int64_t)kC * p.a.HV * p.a.V;
     // of chunks it - 2 and it - 1: e^{G_i}, and this thread's row of o (NULL past the sequence's end)
-    float f = 0.f, f1 = 0.f, f_next = 0.f, unused;
+    float f = 0.f, f1 = 0.f, f_next = 0.f, total;
     __nv_bfloat16 *dst = nullptr, *dst1 = nullptr;
     auto output = [&](uint32_t d) -> bool {
       if (!warp_wait(&sm.o_full, d & 1)) return false;
@@ -632,7 +645,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
           static_cast<__nv_bfloat16*>(p.a.o) + ((t.bos + i) * p.a.HV + t.hv) * p.a.V + 64 * t.z;
       for (int j = 0; j < t.ce - t.cb; ++j, ++it) {
         const int c = nth(j);
-        if (!(ok = weigh(c, i, kHalf, kHalf, f_next, unused))) break;
+        if (!(ok = prepare(c, i, f_next, total) && put(c, i))) break;
         if (it > 1 && !(ok = output(it - 2))) break;
         f = f1;
         dst = dst1;
@@ -1282,12 +1295,12 @@ struct ScanMaps {
   CUtensorMap x, q, y, s;
 };
 
-template <int K, bool kOut, bool kStore, bool kBack, bool kExact>
+template <int K, bool kOut, bool kStore, bool kBack>
 int run_scan(const ScanArgs& p, const ScanMaps& m, cudaStream_t s) {
-  auto kern = la_scan_kernel<K, kOut, kStore, kBack, kExact>;
-  constexpr size_t bytes = sizeof(ScanSmem<K, kOut, kExact>);
+  constexpr auto kern = la_scan_kernel<K, kOut, kStore, kBack>;
+  constexpr size_t bytes = sizeof(ScanSmem<K, kOut>);
   static_assert(bytes <= 227 * 1024, "shared memory of the scan");
-  GDN2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (int st = smem_opt_in<kern>(bytes)) return st;
   ProfScope ps(kOut ? kKLinAttnScan : kKLinAttnStates, s);
   kern<<<(unsigned)std::min<int64_t>(p.tasks, kLaSms), kOut ? 640 : 256, bytes, s>>>(p, m.x, m.q, m.y, m.s);
   GDN2_LAUNCH_CHECK();
@@ -1296,23 +1309,18 @@ int run_scan(const ScanArgs& p, const ScanMaps& m, cudaStream_t s) {
 
 // one direction of the scan: the segments' own states and their sum first where the sequences are cut
 template <int K, bool kBack>
-int scan(ScanArgs& p, const ScanMaps& m, bool out, bool store, bool exact, cudaStream_t s) {
+int scan(ScanArgs& p, const ScanMaps& m, bool store, cudaStream_t s) {
   if (p.seg.multi) {
     p.pre = 1;
-    if (int st = run_scan<K, false, false, kBack, true>(p, m, s)) return st;
+    if (int st = run_scan<K, false, false, kBack>(p, m, s)) return st;
     const int64_t KV = p.a.K * p.a.V;
     la_segment_kernel<kBack><<<dim3((unsigned)(p.a.N * p.a.HV), (unsigned)((KV + 511) / 512)), 128, 0, s>>>(
         p.seg, p.geo, p.a.HV, KV);
     GDN2_LAUNCH_CHECK();
     p.pre = 0;
   }
-  if constexpr (kBack) {
-    return exact ? run_scan<K, false, true, true, true>(p, m, s) : run_scan<K, false, true, true, false>(p, m, s);
-  } else {
-    if (store)
-      return exact ? run_scan<K, true, true, false, true>(p, m, s) : run_scan<K, true, true, false, false>(p, m, s);
-    return exact ? run_scan<K, true, false, false, true>(p, m, s) : run_scan<K, true, false, false, false>(p, m, s);
-  }
+  if constexpr (kBack) return run_scan<K, false, true, true>(p, m, s);
+  else return store ? run_scan<K, true, true, false>(p, m, s) : run_scan<K, true, false, false>(p, m, s);
 }
 
 }  // namespace
@@ -1330,17 +1338,16 @@ int la_tc_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_
     return GDN2_ERR_TENSOR_MAP;
   m.s = m.y;
   if (save && !state_map(&m.s, ws.states16, a.V, la_num_chunks(a) * a.HV * a.K, a.K)) return GDN2_ERR_TENSOR_MAP;
-  const bool exact = a.flags & GDN2_STORE_FINAL;
-  return a.K == 128 ? scan<128, false>(p, m, true, save, exact, s) : scan<64, false>(p, m, true, save, exact, s);
+  return a.K == 128 ? scan<128, false>(p, m, save, s) : scan<64, false>(p, m, save, s);
 }
 
 namespace {
 
 template <int K, int V, bool kDg>
 int run_bwd(const BwdArgs& p, const CUtensorMap (&m)[6], cudaStream_t s) {
-  auto kern = la_bwd_tc_kernel<K, V, kDg>;
+  constexpr auto kern = la_bwd_tc_kernel<K, V, kDg>;
   static_assert(sizeof(BwdSmem) <= 227 * 1024, "shared memory of the backward");
-  GDN2_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(BwdSmem)));
+  if (int st = smem_opt_in<kern>(sizeof(BwdSmem))) return st;
   ProfScope ps(kKLinAttnBwd, s);
   kern<<<(unsigned)std::min<int64_t>(p.items, kLaSms), 384, sizeof(BwdSmem), s>>>(p, m[0], m[1], m[2], m[3], m[4], m[5]);
   GDN2_LAUNCH_CHECK();
@@ -1373,9 +1380,7 @@ int la_tc_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grad
       !state_map(&m[5], bw.dstates16, a.V, rows, a.K))
     return GDN2_ERR_TENSOR_MAP;
   const ScanMaps sm{m[0], m[0], m[3], m[5]};
-  const bool exact = gr.dh0 != nullptr;
-  if (int st = a.K == 128 ? scan<128, true>(sc, sm, false, true, exact, s) : scan<64, true>(sc, sm, false, true, exact, s))
-    return st;
+  if (int st = a.K == 128 ? scan<128, true>(sc, sm, true, s) : scan<64, true>(sc, sm, true, s)) return st;
   if (a.K == 128) return a.V == 128 ? bwd<128, 128>(p, m, s) : bwd<128, 64>(p, m, s);
   return a.V == 128 ? bwd<64, 128>(p, m, s) : bwd<64, 64>(p, m, s);
 }

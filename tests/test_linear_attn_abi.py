@@ -11,8 +11,7 @@ import torch
 def _la(gdn2, **kw):
     L = gdn2._lib
     a = dict(B=2, T=100, H=2, HV=4, K=64, V=128, N=2, scale=0.125, flags=0, dtype=L.BF16, dtype_g=L.F32,
-             decay=L.DECAY_NONE, q_stride=L._s3(12800, 128, 64), k_stride=L._s3(12800, 128, 64),
-             v_stride=L._s3(51200, 512, 128))
+             decay=L.DECAY_NONE, q_b=12800, q_t=128, q_h=64, k_b=12800, k_t=128, k_h=64, v_b=51200, v_t=512, v_h=128)
     a.update(kw)
     return L.LinearAttnArgs(**a)
 
@@ -34,7 +33,7 @@ def test_linear_attn_alignment_workspace_and_flags(gdn2):
     p = (ctypes.addressof(buf) + 15) & ~15
     ptrs = dict(q=p, k=p, v=p, o=p)
     assert lib.gdn2_linear_attn_fwd(_la(gdn2, **{**ptrs, "q": p + 2}), None, 0, None) == 5
-    assert lib.gdn2_linear_attn_fwd(_la(gdn2, **ptrs, v_stride=L._s3(51200, 516, 128)), None, 0, None) == 5
+    assert lib.gdn2_linear_attn_fwd(_la(gdn2, **ptrs, v_t=516), None, 0, None) == 5
     assert lib.gdn2_linear_attn_fwd(_la(gdn2, **ptrs, flags=L.SAVE_FOR_BWD), None, 0, None) == 6
     assert lib.gdn2_linear_attn_workspace_size(_la(gdn2, flags=L.SAVE_FOR_BWD)) >= 2 * 1 * 4 * 64 * 128 * 2
     assert lib.gdn2_linear_attn_workspace_size(_la(gdn2)) == 0  # one segment, nothing kept
