@@ -11,9 +11,12 @@
 // below run through the chunks of all its tasks as one pipeline, so a task's
 // loads overlap the end of the one before.
 //   warp 0      TMA loads (q, k: two stages, three without outputs; v: three)
-//   warp 1      allocates TMEM, issues the MMAs
-//   warp 2      running sums of g in fp64, handed on as pairs of floats
-//   warp 3      TMA stores of the chunks' entering states
+//   warp 1      MMAs: Q K^T of chunk i, P V of chunk i - 1 (P from TMEM)
+//   warp 2      running sums of g in fp64, handed on as a float and what it misses;
+//               TMA stores of the chunks' entering states (without outputs: warp 1)
+//   warp 3      MMAs: K^T (w v) and Q S.  Two issuers: neither chain waits for the other's
+//               barriers, and an issuer ahead of the tensor pipe holds up the memory
+//               instructions of its own quarter of the SM only
 //   warps 4-11  scores (64 columns per four warps): Q K^T out of TMEM, decayed,
 //               back as the bf16 operand P.  Off the diagonal e^{G_i - G_j} =
 //               e^{G_i - G_r} e^{G_r - G_j} with r the first row of the 32-row block:
@@ -22,9 +25,7 @@
 //   warps 12-15 the state in registers (thread = row k of S): S <- e^{G_C} S + what
 //               the MMA left in TMEM; bf16 copy for Q S (without outputs also w v)
 //   warps 16-19 w v; o out of TMEM (thread = token), straight to memory, 32 bytes a store
-// MMA order per chunk i: Q K^T, K^T (w v), then P V of chunk i - 1, then Q S.  The
-// lag gives the scores more than a chunk's time, and a q, k stage is held only
-// from its first product to its last, so two stages cover the loads' latency.
+// P V lags by a chunk, which gives the scores more than a chunk's time.
 // Precision: P and S are rounded to bf16 as MMA operands (as the result itself
 // is).  w v goes in as the sum of two bf16 values, so the fp32 state carries 16
 // bits or more of every product: with one it would hold 8, and o as many again less.
@@ -73,7 +74,7 @@ struct alignas(1024) ScanSmem {
   Sums f[2];
   float cw[kOut ? 320 : 4];  // column factors of the score warps, 32 (w + 1) for w = 0..3
   uint64_t full_x[NX], empty_x[NX], full_y[NY], empty_y[NY], f_full[2], f_empty[2], qk_full[2], p_full[2];
-  uint64_t yw_full[NB], ds_full[NB], ds_free, s_full, s_free, o_full, o_free, aborted;
+  uint64_t yw_full[NB], ds_full[NB], ds_free, s_full, s_free, y_ready[NY], o_full[2], o_free, drained;
   uint32_t tbase;
 };
 
@@ -189,17 +190,19 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
   if (tid == 0) {
     for (uint32_t i = 0; i < NX; ++i) {
       tc::mbar_init(&sm.full_x[i], 1);
-      tc::mbar_init(&sm.empty_x[i], 1);
+      tc::mbar_init(&sm.empty_x[i], kOut ? 2 : 1);  // one per issuer
     }
     for (uint32_t i = 0; i < NY; ++i) {
       tc::mbar_init(&sm.full_y[i], 1);
       tc::mbar_init(&sm.empty_y[i], kOut ? 1 : 128);
+      tc::mbar_init(&sm.y_ready[i], 128);
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sm.f_full[i], 32);
       tc::mbar_init(&sm.f_empty[i], kOut ? 16 : 4);  // one per warp that reads them
       tc::mbar_init(&sm.qk_full[i], 1);
       tc::mbar_init(&sm.p_full[i], 256);
+      tc::mbar_init(&sm.o_full[i], 2);  // Q S and P V
     }
     for (uint32_t i = 0; i < NB; ++i) {
       tc::mbar_init(&sm.yw_full[i], 128);
@@ -208,9 +211,8 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
     tc::mbar_init(&sm.ds_free, 128);
     tc::mbar_init(&sm.s_full, 128);
     tc::mbar_init(&sm.s_free, 1);
-    tc::mbar_init(&sm.o_full, 1);
+    tc::mbar_init(&sm.drained, kOut ? 2 : 1);  // one per issuer
     tc::mbar_init(&sm.o_free, 128);
-    tc::mbar_init(&sm.aborted, 1);
     tc::mbar_fence_init();
   }
   if (warp == 1) tc::tmem_alloc(&sm.tbase, kCols);
@@ -226,6 +228,12 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
   // the token coordinate and batch of chunk c in the tensor maps
   auto tok = [&](int c) { return (int)((p.geo.cu ? t.bos : 0) + (int64_t)c * kC); };
   const int64_t step = gridDim.x;
+  auto count_chunks = [&]() {  // over all tasks
+    uint32_t n = 0;
+    for (int64_t id = blockIdx.x; id < p.tasks; id += step)
+      if (find_task<kBack>(p, id, t)) n += (uint32_t)max(t.ce - t.cb, 0);
+    return n;
+  };
   // w v of chunk `it`, row j of its tile (token j): made in registers, so that it can
   // be ready before the MMAs have read the chunk before's, then put in shared memory.
   // f_row: e^{G_j}, total: e^{G_C}.
@@ -286,7 +294,8 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
     }
     tc::fence_proxy_async();
     tc::mbar_arrive(&sm.yw_full[b]);
-    if constexpr (!kOut) tc::mbar_arrive(&sm.empty_y[sy]);
+    if constexpr (kOut) tc::mbar_arrive(&sm.y_ready[sy]);  // landed, and clear of other sequences' rows
+    else tc::mbar_arrive(&sm.empty_y[sy]);
     return true;
   };
 
@@ -324,76 +333,101 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       }
     }
   } else if (warp == 1) {
-    // ----------------------------------------------------------------- MMAs
-    if (tc::elect_one()) {
+    // ---------------------- MMAs: Q K^T, P V; without outputs: entering states out
+    if constexpr (!kOut) {
+      if (kStore && lane == 0) {
+        for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
+          if (!find_task<kBack>(p, id, t)) continue;
+          for (int i = 0; i < t.ce - t.cb; ++i, ++it) {
+            if (!(ok = wait(&sm.s_full, it & 1))) break;
+            tc::tma_store_2d(&tmS, sm.S, 64 * t.z, (int)(((t.chunk0 + nth(i)) * p.a.HV + t.hv) * K));
+            tc::bulk_commit();
+            tc::bulk_wait_read_all();
+            tc::mbar_arrive(&sm.s_free);
+          }
+        }
+        tc::bulk_wait_all();
+      }
+    } else if (tc::elect_one()) {
       constexpr uint32_t iQK = tc::idesc_bf16(128, 128, 0, 0), iNV = tc::idesc_bf16(128, 64, 0, 1);
-      constexpr uint32_t iDS = tc::idesc_bf16(K, 64, 1, 1);
-      const uint32_t aX = addr16(sm.X), aY = addr16(sm.Y), aW = addr16(sm.YW), aS = addr16(sm.S);
-      // MMAs of 16 along k, one after the other
-      auto mmas = [&](auto steps, auto issue) {
-#pragma unroll
-        for (int kk = 0; kk < steps; ++kk) issue(kk);
-      };
-      constexpr std::integral_constant<int, K / 16> kSteps{};
-      constexpr std::integral_constant<int, 8> tSteps{};  // over the tokens
-      uint32_t total = 0;  // chunks over all tasks
-      for (int64_t id = blockIdx.x; id < p.tasks; id += step)
-        if (find_task<kBack>(p, id, t)) total += (uint32_t)max(t.ce - t.cb, 0);
-      for (; it < total + (kOut && total > 0 ? 1 : 0); ++it) {
-        const uint32_t s = it & 1, sx = it % NX, b = it % NB;
-        const uint32_t ax = aX + sx * (uint32_t)(sizeof(sm.X[0]) >> 4), aq = ax + (K / 64) * (kTile >> 4);
+      const uint32_t aX = addr16(sm.X), aY = addr16(sm.Y), total = count_chunks();
+      for (; it < total + (total > 0 ? 1 : 0); ++it) {
+        const uint32_t s = it & 1, sx = it % NX;
         if (it < total) {
+          const uint32_t ax = aX + sx * (uint32_t)(sizeof(sm.X[0]) >> 4), aq = ax + (K / 64) * (kTile >> 4);
           if (!(ok = wait(&sm.full_x[sx], (it / NX) & 1))) break;
-          if constexpr (kOut) {
-            tc::tc_fence_after();
-            mmas(kSteps, [&](int kk) {
-              tc::mma_bf16(tb + kColQK + 128 * s, kmaj(aq, kk), kmaj(ax, kk), iQK, kk > 0);
-            });
-            tc::mma_commit(&sm.qk_full[s]);
-          }
-          if (!(ok = wait(&sm.yw_full[b], (it / NB) & 1))) break;
-          if constexpr (kOut) {  // the state term of the chunk before has left TMEM
-            if (it > 0 && !(ok = wait(&sm.ds_free, (it - 1) & 1))) break;
-          }
           tc::tc_fence_after();
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            mmas(tSteps, [&](int kk) {
-              tc::mma_bf16(tb + kColDS + 64 * b, nmaj(ax, kk), nmaj(aW + (2 * b + e) * (kTile >> 4), kk), iDS, e + kk > 0);
-            });
-          tc::mma_commit(&sm.ds_full[b]);
-          if constexpr (!kOut) tc::mma_commit(&sm.empty_x[sx]);
+          for (int kk = 0; kk < K / 16; ++kk)
+            tc::mma_bf16(tb + kColQK + 128 * s, kmaj(aq, kk), kmaj(ax, kk), iQK, kk > 0);
+          tc::mma_commit(&sm.qk_full[s]);
+          tc::mma_commit(&sm.empty_x[sx]);
         }
-        if constexpr (kOut) {
-          // chunk it - 2's outputs have left TMEM
-          if (it >= 2 && !(ok = wait(&sm.o_free, it & 1))) break;
-          if (it > 0) {
-            const uint32_t j = it - 1, sj = j & 1, sy = j % NY;
-            if (!(ok = wait(&sm.full_y[sy], (j / NY) & 1) && wait(&sm.p_full[sj], (j >> 1) & 1))) break;
-            tc::tc_fence_after();
-            mmas(tSteps, [&](int kk) {  // P: columns 0-31 and 64-95 of the score buffer
-              tc::mma_bf16_ts(tb + kColO2, tb + kColQK + 128 * sj + 8 * kk + (kk < 4 ? 0 : 32),
-                              nmaj(aY + sy * (kTile >> 4), kk), iNV, kk > 0);
-            });
-            tc::mma_commit(&sm.o_full);
-            tc::mma_commit(&sm.empty_y[sy]);
-          }
-          if (it < total) {
-            if (!(ok = wait(&sm.s_full, it & 1))) break;
-            tc::tc_fence_after();
-            mmas(kSteps, [&](int kk) {
-              tc::mma_bf16(tb + kColO1 + 64 * s, kmaj(aq, kk), nmaj(aS, kk), iNV, kk > 0);
-            });
-            tc::mma_commit(&sm.empty_x[sx]);  // also: S has been read
-          }
+        if (it > 0) {
+          const uint32_t j = it - 1, sj = j & 1, sy = j % NY;
+          if (j > 0 && !(ok = wait(&sm.o_free, (j - 1) & 1))) break;  // P V of the chunk before has left TMEM
+          if (!(ok = wait(&sm.y_ready[sy], (j / NY) & 1) && wait(&sm.p_full[sj], (j >> 1) & 1))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)  // P: columns 0-31 and 64-95 of the score buffer
+            tc::mma_bf16_ts(tb + kColO2, tb + kColQK + 128 * sj + 8 * kk + (kk < 4 ? 0 : 32),
+                            nmaj(aY + sy * (kTile >> 4), kk), iNV, kk > 0);
+          tc::mma_commit(&sm.o_full[sj]);
+          tc::mma_commit(&sm.empty_y[sy]);
         }
       }
-      // what was issued has completed before TMEM is released
-      tc::mma_commit(&sm.aborted);
-      if (!wait(&sm.aborted, 0)) ok = false;
+      tc::mma_commit(&sm.drained);  // what was issued has completed before TMEM is released
+      if (!wait(&sm.drained, 0)) ok = false;
+    }
+  } else if (warp == 3) {
+    // --------------------------------------------- MMAs: K^T (w v), Q S
+    if (tc::elect_one()) {
+      constexpr uint32_t iNV = tc::idesc_bf16(128, 64, 0, 1), iDS = tc::idesc_bf16(K, 64, 1, 1);
+      const uint32_t aX = addr16(sm.X), aW = addr16(sm.YW), aS = addr16(sm.S), total = count_chunks();
+      for (; it < total; ++it) {
+        const uint32_t s = it & 1, sx = it % NX, b = it % NB;
+        const uint32_t ax = aX + sx * (uint32_t)(sizeof(sm.X[0]) >> 4), aq = ax + (K / 64) * (kTile >> 4);
+        if (!(ok = wait(&sm.full_x[sx], (it / NX) & 1) && wait(&sm.yw_full[b], (it / NB) & 1))) break;
+        if constexpr (kOut) {  // the state term of the chunk before has left TMEM
+          if (it > 0 && !(ok = wait(&sm.ds_free, (it - 1) & 1))) break;
+        }
+        tc::tc_fence_after();
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            tc::mma_bf16(tb + kColDS + 64 * b, nmaj(ax, kk), nmaj(aW + (2 * b + e) * (kTile >> 4), kk), iDS, e + kk > 0);
+        tc::mma_commit(&sm.ds_full[b]);
+        if constexpr (kOut) {
+          if (it >= 2 && !(ok = wait(&sm.o_free, it & 1))) break;  // Q S of two chunks before has left TMEM
+          if (!(ok = wait(&sm.s_full, it & 1))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < K / 16; ++kk)
+            tc::mma_bf16(tb + kColO1 + 64 * s, kmaj(aq, kk), nmaj(aS, kk), iNV, kk > 0);
+          tc::mma_commit(&sm.o_full[s]);
+        }
+        tc::mma_commit(&sm.empty_x[sx]);  // also: S has been read
+      }
+      tc::mma_commit(&sm.drained);
+      if (!wait(&sm.drained, 0)) ok = false;
     }
   } else if (warp == 2) {
-    // ---------------------------------------------------------------- sums
+    // ---------------------------- sums; with outputs also the entering states out
+    constexpr bool kStoreHere = kOut && kStore;
+    // (the sums run ahead of the states, so each turn stores the one of two chunks before)
+    int out_row[2] = {0, 0}, out_z[2] = {0, 0};
+    auto store = [&](uint32_t d) -> bool {
+      if (!warp_wait(&sm.s_full, d & 1)) return false;
+      if (lane == 0) {
+        tc::tma_store_2d(&tmS, sm.S, 64 * (d & 1 ? out_z[1] : out_z[0]), d & 1 ? out_row[1] : out_row[0]);
+        tc::bulk_commit();
+        tc::bulk_wait_read_all();
+        tc::mbar_arrive(&sm.s_free);
+      }
+      __syncwarp();
+      return true;
+    };
     for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
       // this lane's four tokens of a chunk lie `gs` bytes apart (0: one decay for all)
@@ -436,27 +470,25 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
           lo[e] = (float)(G[e] - (double)hi[e]);
         }
         if (p.pre) sum += __shfl_sync(0xffffffffu, inc, 31);
+        if constexpr (kStoreHere) {
+          if (it >= 2 && !(ok = store(it - 2))) break;
+        }
         if (it >= 2 && !(ok = warp_wait(&sm.f_empty[s], ((it >> 1) & 1) ^ 1))) break;
         reinterpret_cast<float4*>(sm.f[s].hi)[lane] = make_float4(hi[0], hi[1], hi[2], hi[3]);
         reinterpret_cast<uint2*>(sm.f[s].lo)[lane] = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
         tc::mbar_arrive(&sm.f_full[s]);
+        if constexpr (kStoreHere) {
+          const int r = (int)(((t.chunk0 + nth(i)) * p.a.HV + t.hv) * K);
+          if (s) out_row[1] = r, out_z[1] = t.z;
+          else out_row[0] = r, out_z[0] = t.z;
+        }
       }
       if (p.pre && lane == 0 && t.z == 0) p.seg.D[t.entry * p.a.HV + t.hv] = expf((float)sum);
     }
-  } else if (warp == 3) {
-    // --------------------------------------------------------------- stores
-    if (lane == 0 && kStore) {
-      for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
-        if (!find_task<kBack>(p, id, t)) continue;
-        for (int i = 0; i < t.ce - t.cb; ++i, ++it) {
-          if (!(ok = wait(&sm.s_full, it & 1))) break;
-          tc::tma_store_2d(&tmS, sm.S, 64 * t.z, (int)(((t.chunk0 + nth(i)) * p.a.HV + t.hv) * K));
-          tc::bulk_commit();
-          tc::bulk_wait_read_all();
-          tc::mbar_arrive(&sm.s_free);
-        }
-      }
-      tc::bulk_wait_all();
+    if constexpr (kStoreHere) {
+      if (ok && it > 1) ok = store(it - 2);
+      if (ok && it > 0) ok = store(it - 1);
+      if (lane == 0) tc::bulk_wait_all();
     }
   } else if (kOut && warp < 12) {
     // --------------------------------------------------------------- scores
@@ -621,7 +653,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
     float f = 0.f, f1 = 0.f, f_next = 0.f, total;
     __nv_bfloat16 *dst = nullptr, *dst1 = nullptr;
     auto output = [&](uint32_t d) -> bool {
-      if (!warp_wait(&sm.o_full, d & 1)) return false;
+      if (!warp_wait(&sm.o_full[d & 1], (d >> 1) & 1)) return false;
       tc::tc_fence_after();
       const uint64_t f2 = tc::mul2(sc2, tc::pack2(f, f));
 #pragma unroll 1
