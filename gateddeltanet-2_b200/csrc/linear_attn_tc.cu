@@ -765,7 +765,7 @@ GDN2_DEV float dot16(const unsigned char* row_base, int p0, int row, const float
 // next chunk's tile (x + 3) % 6 as soon as it has been read, so v, S and dS' make
 // room for q, k and do of the next chunk while this one is being finished.
 //   warp 0 loads, warp 1 MMAs, warp 2 running sums, warp 3 dg,
-//   warps 4-11: thread = token (TMEM lane) and one half of the columns
+//   warps 4-19: thread = token (TMEM lane) and a quarter of the columns
 // ---------------------------------------------------------------------------
 enum Tile { kTQ = 0, kTK, kTO, kTV, kTS, kTD };  // q, k, do, v, S, dS'
 
@@ -775,8 +775,8 @@ struct alignas(1024) BwdSmem {
   float hi[kC];                  // running sums of g
   float g2[kC];                  // (G_i - G_{32 floor(i / 32)}) log2 e
   float r[kC];                   // 2^g2
-  float xy[2][kC];               // X - Y, per half of the columns
-  float part[16];                // per warp: sum of k . dk (state part), e^{G_C} <S, dS'>
+  float xy[2][kC];               // X - Y, per half of the columns (two terms on a zero: their order is nothing)
+  float part[32];                // per warp: sum of k . dk (state part), e^{G_C} <S, dS'>
   uint64_t full[6], empty[6], f_full, f_empty, clean, g1, g2_, pe, rmw1, g3, rmw2, g4a, g4b, qk_free, dv_free, xy_full,
       xy_free, aborted;
   uint32_t tbase;
@@ -793,7 +793,7 @@ struct BwdArgs {
 };
 
 template <int K, int V, bool kDg>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(640, 1)
 la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUtensorMap tmQ,
                  const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmS,
@@ -805,26 +805,27 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
   if (tid == 0) {
     for (int i = 0; i < 6; ++i) {
       tc::mbar_init(&sm.full[i], 1);
-      tc::mbar_init(&sm.empty[i], 9);  // the MMAs' commit and the eight row warps
+      tc::mbar_init(&sm.empty[i], 17);  // the MMAs' commit and the row warps
     }
     tc::mbar_init(&sm.f_full, 32);
-    tc::mbar_init(&sm.f_empty, 8);
-    tc::mbar_init(&sm.clean, 256);
+    tc::mbar_init(&sm.f_empty, 16);
+    tc::mbar_init(&sm.clean, 512);
     tc::mbar_init(&sm.g1, 1);
     tc::mbar_init(&sm.g2_, 1);
-    tc::mbar_init(&sm.pe, 256);
-    tc::mbar_init(&sm.rmw1, 256);
+    tc::mbar_init(&sm.pe, 512);
+    tc::mbar_init(&sm.rmw1, 512);
     tc::mbar_init(&sm.g3, 1);
-    tc::mbar_init(&sm.rmw2, 256);
+    tc::mbar_init(&sm.rmw2, 512);
     tc::mbar_init(&sm.g4a, 1);
     tc::mbar_init(&sm.g4b, 1);
-    tc::mbar_init(&sm.qk_free, 256);
-    tc::mbar_init(&sm.dv_free, 256);
-    tc::mbar_init(&sm.xy_full, 256);
+    tc::mbar_init(&sm.qk_free, 512);
+    tc::mbar_init(&sm.dv_free, 512);
+    tc::mbar_init(&sm.xy_full, 512);
     tc::mbar_init(&sm.xy_free, 32);
     tc::mbar_init(&sm.aborted, 1);
     tc::mbar_fence_init();
   }
+  if (tid < 2 * kC) sm.xy[0][tid] = 0.f;
   if (warp == 1) tc::tmem_alloc(&sm.tbase, 512);
   tc::tc_fence_before();
   __syncthreads();
@@ -943,7 +944,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           for (int kk = 0; kk < 8; ++kk) tc::mma_bf16(tb + kColDq, nmaj(aE, kk), nmaj(ak, kk), iKmn, 1);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            tc::mma_bf16_ts(tb + kColDk, tb + kColA1 + 64 * (kk >> 2) + 32 + 8 * (kk & 3), nmaj(aq, kk), iKn, 1);
+            tc::mma_bf16_ts(tb + kColDk, tb + kColA1 + 32 * (kk >> 1) + 16 + 8 * (kk & 1), nmaj(aq, kk), iKn, 1);
           tc::mma_commit(&sm.g4a);
           tc::mma_commit(&sm.empty[slot_of(kTQ)]);
           tc::mma_commit(&sm.empty[slot_of(kTK)]);
@@ -951,7 +952,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           tc::tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            tc::mma_bf16_ts(tb + kColA2, tb + kColA1 + 64 * (kk >> 2) + 8 * (kk & 3), nmaj(ao, kk), iVn, 1);
+            tc::mma_bf16_ts(tb + kColA2, tb + kColA1 + 32 * (kk >> 1) + 8 * (kk & 1), nmaj(ao, kk), iVn, 1);
           tc::mma_commit(&sm.g4b);
           tc::mma_commit(&sm.empty[slot_of(kTO)]);
         }
@@ -1004,7 +1005,9 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           if (!(ok = warp_wait(&sm.xy_full, n & 1))) break;
           const float4 x0 = reinterpret_cast<const float4*>(sm.xy[0])[lane];
           const float4 x1 = reinterpret_cast<const float4*>(sm.xy[1])[lane];
-          float base = lane < 16 ? sm.part[lane] : 0.f;
+          float base = sm.part[lane];
+          reinterpret_cast<float4*>(sm.xy[0])[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+          reinterpret_cast<float4*>(sm.xy[1])[lane] = make_float4(0.f, 0.f, 0.f, 0.f);
           __syncwarp();
           tc::mbar_arrive(&sm.xy_free);
           float d[4] = {x0.x + x1.x, x0.y + x1.y, x0.z + x1.z, x0.w + x1.w};
@@ -1038,10 +1041,10 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
     }
   } else {
     // ----------------------------------------------------------------- rows
-    const int q4 = warp & 3, row = 32 * q4 + lane, half = (warp - 4) >> 2;
+    const int q4 = warp & 3, row = 32 * q4 + lane, quarter = (warp - 4) >> 2;
     const uint32_t tl = tb + ((uint32_t)(32 * q4) << 16);
     const int64_t H = p.a.H, HV = p.a.HV;
-    float* acc = p.acc + ((int64_t)blockIdx.x * 2 * kC + row) * K + half * (K / 2);
+    float* acc = p.acc + ((int64_t)blockIdx.x * 2 * kC + row) * K + quarter * (K / 4);
     for (int64_t id = blockIdx.x; id < p.items && ok; id += step) {
       if (!witem(id)) continue;
       const int64_t tok = w.bos + w.c * kC + row;
@@ -1062,9 +1065,9 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           if (!inside) {
 #pragma unroll 1
             for (int x = kTQ; x <= kTV; ++x) {
-              if ((x <= kTK ? K : V) == 64 && half) continue;  // 64-column blocks: one per half
-              uint4* dst = reinterpret_cast<uint4*>(tile(x) + half * kTile + row * 128);
-              for (int e = 0; e < 8; ++e) dst[e] = make_uint4(0, 0, 0, 0);
+              if ((x <= kTK ? K : V) == 64 && quarter > 1) continue;  // a block of 64 columns: two quarters
+              uint4* dst = reinterpret_cast<uint4*>(tile(x) + (quarter >> 1) * kTile + row * 128) + 4 * (quarter & 1);
+              for (int e = 0; e < 4; ++e) dst[e] = make_uint4(0, 0, 0, 0);
             }
           }
           tc::fence_proxy_async();
@@ -1074,54 +1077,53 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         const float hj = sm.hi[row], gj = sm.g2[row], gc = sm.hi[kC - 1];
         const float out_f = p.a.scale * exp_of(hj), in_f = exp_of(gc - hj);  // of the products with S and dS'
         const float eGC = exp_of(gc);
-        float block_f[2];  // e^{G_{32 I} - G_j} scale of this half's two 32-column blocks (I > q4)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) block_f[e] = p.a.scale * exp_of(sm.hi[64 * half + 32 * e] - hj);
+        const float block_f = p.a.scale * exp_of(sm.hi[32 * quarter] - hj);  // of the 32 columns where quarter > q4
         if (!(ok = warp_wait(&sm.g1, par))) break;
         tc::tc_fence_after();
         // ---- P^T, E^T ------------------------------------------------------
         {
-          float a1[4][16];
+          const uint32_t cs = tl + kColA1 + 32 * quarter;
+          unsigned char* erow = reinterpret_cast<unsigned char*>(sm.E[quarter >> 1]) + row * 128;
+          float a1[2][16];  // both before the first store: E^T lands on the second one's columns
+          if (quarter >= q4) {
 #pragma unroll
-          for (int b = 0; b < 4; ++b) tc::tmem_ld16(tl + kColA1 + 64 * half + 16 * b, a1[b]);
-          unsigned char* erow = reinterpret_cast<unsigned char*>(sm.E[half]) + row * 128;
-          tc::tmem_wait_ld();
+            for (int b = 0; b < 2; ++b) tc::tmem_ld16(cs + 16 * b, a1[b]);
+          }
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const int c0 = 64 * half + 16 * b, d0 = c0 - 32 * q4;  // first column i, and its place from the diagonal block
+          for (int b = 0; b < 2; ++b) {
+            const int c0 = 32 * quarter + 16 * b;
             uint32_t pp[8], ee[8];
-            if (d0 < 0) {
+            if (quarter < q4) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) pp[e] = ee[e] = 0;
             } else {
               float a2[16];
               tc::tmem_ld16(tl + kColA2 + c0, a2);
-              float f[16];
-              if (d0 >= 32) {
-                const float bf = block_f[b >> 1];
-                const float4* rr = reinterpret_cast<const float4*>(sm.r + c0);
+              tc::tmem_wait_ld();
+              if (quarter > q4) {
+                const uint64_t* rr = reinterpret_cast<const uint64_t*>(sm.r + c0);
+                const uint64_t bf2 = tc::pack2(block_f, block_f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float4 x = rr[e];
-                  f[4 * e] = x.x * bf; f[4 * e + 1] = x.y * bf; f[4 * e + 2] = x.z * bf; f[4 * e + 3] = x.w * bf;
+                for (int e = 0; e < 16; e += 2) {
+                  const uint64_t f2 = tc::mul2(rr[e / 2], bf2);
+                  tc::unpack2(tc::mul2(tc::pack2(a1[b][e], a1[b][e + 1]), f2), a1[b][e], a1[b][e + 1]);
+                  tc::unpack2(tc::mul2(tc::pack2(a2[e], a2[e + 1]), f2), a2[e], a2[e + 1]);
                 }
               } else {
                 const float4* gg = reinterpret_cast<const float4*>(sm.g2 + c0);
-                const int first = lane - d0;  // columns from this one on are not in the past
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float4 x = gg[e];
                   const float y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                  for (int u = 0; u < 4; ++u) f[4 * e + u] = 4 * e + u >= first ? p.a.scale * exp2_approx(y[u] - gj) : 0.f;
+                  for (int u = 0; u < 4; ++u) {  // (a select: what lies in the past may not be finite)
+                    const int i = 4 * e + u;
+                    const float f = p.a.scale * exp2_approx(y[u] - gj);
+                    const bool keep = 16 * b + i >= lane;
+                    a1[b][i] = keep ? a1[b][i] * f : 0.f;
+                    a2[i] = keep ? a2[i] * f : 0.f;
+                  }
                 }
-              }
-              tc::tmem_wait_ld();
-              const int first = d0 >= 32 ? 0 : lane - d0;
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {  // (a select: what lies in the past may not be finite)
-                a1[b][e] = e >= first ? a1[b][e] * f[e] : 0.f;
-                a2[e] = e >= first ? a2[e] * f[e] : 0.f;
               }
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
@@ -1129,11 +1131,11 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
                 ee[e] = pack_bf16(a2[2 * e], a2[2 * e + 1]);
               }
             }
-            tc::tmem_st8(tl + kColA1 + 64 * half + 8 * b, pp);
-            tc::tmem_st8(tl + kColA1 + 64 * half + 32 + 8 * b, ee);
+            tc::tmem_st8(cs + 8 * b, pp);
+            tc::tmem_st8(cs + 16 + 8 * b, ee);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<uint4*>(erow + (((2 * b + e) ^ (row & 7)) << 4)) =
+              *reinterpret_cast<uint4*>(erow + (((4 * (quarter & 1) + 2 * b + e) ^ (row & 7)) << 4)) =
                   make_uint4(ee[4 * e], ee[4 * e + 1], ee[4 * e + 2], ee[4 * e + 3]);
           }
           tc::tmem_wait_st();
@@ -1147,15 +1149,15 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         if (!(ok = warp_wait(&sm.g2_, par))) break;
         tc::tc_fence_after();
         float kin = 0.f, sdot = 0.f;
-        const unsigned char* krow = tile(kTK) + (K == 128 ? half * kTile : 0) + row * 128;
-        const unsigned char* qrow = tile(kTQ) + (K == 128 ? half * kTile : 0) + row * 128;
-        constexpr int kTurns = K / 32;  // of 16 columns, per half
-        const int p0 = K == 128 ? 0 : 4 * half;  // first 16-byte piece of this half's columns in the row
+        const unsigned char* krow = tile(kTK) + (K == 128 ? (quarter >> 1) * kTile : 0) + row * 128;
+        const unsigned char* qrow = tile(kTQ) + (K == 128 ? (quarter >> 1) * kTile : 0) + row * 128;
+        constexpr int kTurns = K / 64;  // of 16 columns, per quarter
+        const int p0 = K == 128 ? 4 * (quarter & 1) : 2 * quarter;  // first 16-byte piece of these columns in the row
         const uint64_t of2 = tc::pack2(out_f, out_f), if2 = tc::pack2(in_f, in_f);
 #pragma unroll 1
         for (int b = 0; b < kTurns; ++b) {
           float x[16], y[16];
-          const uint32_t cq = tl + kColDq + half * (K / 2) + 16 * b, ck = tl + kColDk + half * (K / 2) + 16 * b;
+          const uint32_t cq = tl + kColDq + quarter * (K / 4) + 16 * b, ck = tl + kColDk + quarter * (K / 4) + 16 * b;
           tc::tmem_ld16(cq, x);
           tc::tmem_ld16(ck, y);
           tc::tmem_wait_ld();
@@ -1172,7 +1174,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           const uint4* s4 = reinterpret_cast<const uint4*>(tile(kTS));
           const uint4* d4 = reinterpret_cast<const uint4*>(tile(kTD));
 #pragma unroll 2
-          for (int e = tid - 128; e < K * V / 8; e += 256) sdot += dot8(s4[e], d4[e]);
+          for (int e = tid - 128; e < K * V / 8; e += 512) sdot += dot8(s4[e], d4[e]);
           sdot *= eGC;
         }
         tc::tmem_wait_st();
@@ -1185,9 +1187,9 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         if (!(ok = warp_wait(&sm.g3, par))) break;
         tc::tc_fence_after();
 #pragma unroll 1
-        for (int b = 0; b < V / 32; ++b) {
+        for (int b = 0; b < V / 64; ++b) {
           float x[16];
-          const uint32_t cv = tl + kColA2 + half * (V / 2) + 16 * b;
+          const uint32_t cv = tl + kColA2 + quarter * (V / 4) + 16 * b;
           tc::tmem_ld16(cv, x);
           tc::tmem_wait_ld();
 #pragma unroll
@@ -1203,12 +1205,12 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         float xy = 0.f;
 #pragma unroll 1
         for (int z = 0; z < 2; ++z) {  // dq, dk
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(z ? p.gr.dk : p.gr.dq) + (tok * H + w.h) * K + half * (K / 2);
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(z ? p.gr.dk : p.gr.dq) + (tok * H + w.h) * K + quarter * (K / 4);
           float* sum = acc + (int64_t)z * kC * K;
 #pragma unroll 1
           for (int b = 0; b < kTurns; ++b) {
             float x[16];
-            tc::tmem_ld16(tl + (z ? kColDk : kColDq) + half * (K / 2) + 16 * b, x);
+            tc::tmem_ld16(tl + (z ? kColDk : kColDq) + quarter * (K / 4) + 16 * b, x);
             tc::tmem_wait_ld();
             if constexpr (kDg) {
               const float d = dot16(z ? krow : qrow, p0 + 2 * b, row, x);
@@ -1236,11 +1238,11 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         tc::mbar_arrive(&sm.qk_free);
         if (!(ok = warp_wait(&sm.g4b, par))) break;
         tc::tc_fence_after();
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.gr.dv) + (tok * HV + hv) * V + half * (V / 2);
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.gr.dv) + (tok * HV + hv) * V + quarter * (V / 4);
 #pragma unroll 1
-        for (int b = 0; b < V / 32; ++b) {
+        for (int b = 0; b < V / 64; ++b) {
           float x[16];
-          tc::tmem_ld16(tl + kColA2 + half * (V / 2) + 16 * b, x);
+          tc::tmem_ld16(tl + kColA2 + quarter * (V / 4) + 16 * b, x);
           tc::tmem_wait_ld();
           if (inside) st_32bytes(out + 16 * b, pack8(x), pack8(x + 8));
         }
@@ -1248,7 +1250,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         tc::mbar_arrive(&sm.dv_free);
         if constexpr (kDg) {
           if (n > 0 && !(ok = warp_wait(&sm.xy_free, (n - 1) & 1))) break;
-          sm.xy[half][row] = xy;
+          atomicAdd(&sm.xy[quarter >> 1][row], xy);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) {
             kin += __shfl_xor_sync(0xffffffffu, kin, o);
@@ -1256,7 +1258,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           }
           if (lane == 0) {
             sm.part[warp - 4] = kin;
-            sm.part[warp + 4] = sdot;
+            sm.part[warp + 12] = sdot;
           }
           tc::mbar_arrive(&sm.xy_full);
         }
@@ -1381,7 +1383,7 @@ int run_bwd(const BwdArgs& p, const CUtensorMap (&m)[6], cudaStream_t s) {
   static_assert(sizeof(BwdSmem) <= 227 * 1024, "shared memory of the backward");
   if (int st = smem_opt_in<kern>(sizeof(BwdSmem))) return st;
   ProfScope ps(kKLinAttnBwd, s);
-  kern<<<(unsigned)std::min<int64_t>(p.items, kLaSms), 384, sizeof(BwdSmem), s>>>(p, m[0], m[1], m[2], m[3], m[4], m[5]);
+  kern<<<(unsigned)std::min<int64_t>(p.items, kLaSms), 640, sizeof(BwdSmem), s>>>(p, m[0], m[1], m[2], m[3], m[4], m[5]);
   GDN2_LAUNCH_CHECK();
   return 0;
 }
