@@ -761,10 +761,10 @@ GDN2_DEV float dot16(const unsigned char* row_base, int p0, int row, const float
 // chunk use the same bf16 E and so cancel where they must,
 //     dg_t = sum_{i>=t} (X_i - Y_i) + sum_j k_j . (e^{G_C - G_j} v_j dS'^T) + e^{G_C} <S, dS'>.
 // A sequence's first token without an initial state decays nothing: exactly zero.
-// Shared memory holds one chunk's six tiles and E^T; a tile's slot goes to the
-// next chunk's tile (x + 3) % 6 as soon as it has been read, so v, S and dS' make
-// room for q, k and do of the next chunk while this one is being finished.
-//   warp 0 loads, warp 1 MMAs, warp 2 running sums, warp 3 dg,
+// Y's part from within the chunk is sum_i E_ij (k_j . q_i), taken from the scores as they are weighed, so that
+// k is not read again.  Shared memory holds one chunk's six tiles and E^T; S, v and dS' make room for the next
+// chunk's q, k and do while this one is being finished, then k, q and do for its v, S and dS'.
+//   warp 0 loads, warp 1 dg, warp 2 running sums, warp 3 MMAs,
 //   warps 4-19: thread = token (TMEM lane) and a quarter of the columns
 // ---------------------------------------------------------------------------
 enum Tile { kTQ = 0, kTK, kTO, kTV, kTS, kTD };  // q, k, do, v, S, dS'
@@ -856,7 +856,8 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
     w.L = uniform(w.L);
     return any;
   };
-  auto slot_of = [&](int x) -> int { return (n & 1) ? (x < 3 ? x + 3 : x - 3) : x; };
+  // q <-> S, k <-> v, do <-> dS' from one pair to the next
+  auto slot_of = [&](int x) -> int { return (n & 1) ? (int)((0x201534u >> (4 * x)) & 7) : x; };
   const int64_t step = gridDim.x;
 
   if (warp == 0) {
@@ -894,9 +895,10 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           wait(&sm.full[s], (n + 1) & 1);
         }
     }
-  } else if (warp == 1) {
+  } else if (warp == 3) {
     // ----------------------------------------------------------------- MMAs
     if (tc::elect_one()) {
+      constexpr int kRoll = 4;
       constexpr uint32_t iA = tc::idesc_bf16(128, 128, 0, 0), iK = tc::idesc_bf16(128, K, 0, 0);
       constexpr uint32_t iVn = tc::idesc_bf16(128, V, 0, 1), iKn = tc::idesc_bf16(128, K, 0, 1);
       constexpr uint32_t iKmn = tc::idesc_bf16(128, K, 1, 1);
@@ -911,21 +913,23 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           auto full = [&](int x) { return wait(&sm.full[slot_of(x)], par); };
           if (!(ok = full(kTQ) && full(kTK) && wait(&sm.clean, par))) break;
           tc::tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < K / 16; ++kk) tc::mma_bf16(tb + kColA1, kmaj(ak, kk), kmaj(aq, kk), iA, kk > 0);
+#pragma unroll kRoll
+          for (int kk = 0; kk < K / 16; ++kk)
+            tc::mma_bf16(tb + kColA1, kmaj(ak, kk), kmaj(aq, kk), iA, kk > 0);
           if (!(ok = full(kTO) && full(kTV) && (n == 0 || wait(&sm.dv_free, prev)))) break;
           tc::tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < V / 16; ++kk) tc::mma_bf16(tb + kColA2, kmaj(av, kk), kmaj(ao, kk), iA, kk > 0);
+#pragma unroll kRoll
+          for (int kk = 0; kk < V / 16; ++kk)
+            tc::mma_bf16(tb + kColA2, kmaj(av, kk), kmaj(ao, kk), iA, kk > 0);
           tc::mma_commit(&sm.g1);
           if (!(ok = full(kTS) && (n == 0 || wait(&sm.qk_free, prev)))) break;
           tc::tc_fence_after();
-#pragma unroll
+#pragma unroll kRoll
           for (int kk = 0; kk < V / 16; ++kk)
             tc::mma_bf16(tb + kColDq, kmaj(ao, kk), desc(as + (kk >> 2) * kBlk + (kk & 3) * 2 + (1u << 16)), iK, kk > 0);
           if (!(ok = full(kTD))) break;
           tc::tc_fence_after();
-#pragma unroll
+#pragma unroll kRoll
           for (int kk = 0; kk < V / 16; ++kk)
             tc::mma_bf16(tb + kColDk, kmaj(av, kk), desc(ad + (kk >> 2) * kBlk + (kk & 3) * 2 + (1u << 16)), iK, kk > 0);
           tc::mma_commit(&sm.g2_);
@@ -933,25 +937,26 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           tc::mma_commit(&sm.empty[slot_of(kTS)]);
           if (!(ok = wait(&sm.pe, par))) break;
           tc::tc_fence_after();
-#pragma unroll
+#pragma unroll kRoll
           for (int kk = 0; kk < K / 16; ++kk)
             tc::mma_bf16(tb + kColA2, kmaj(ak, kk), desc(ad + kk * 128 + (kBlk << 16)), iVn, kk > 0);
           tc::mma_commit(&sm.g3);
           tc::mma_commit(&sm.empty[slot_of(kTD)]);
           if (!(ok = wait(&sm.rmw1, par))) break;
           tc::tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) tc::mma_bf16(tb + kColDq, nmaj(aE, kk), nmaj(ak, kk), iKmn, 1);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
+#pragma unroll kRoll
+          for (int kk = 0; kk < 128 / 16; ++kk)
+            tc::mma_bf16(tb + kColDq, nmaj(aE, kk), nmaj(ak, kk), iKmn, 1);
+#pragma unroll kRoll
+          for (int kk = 0; kk < 128 / 16; ++kk)
             tc::mma_bf16_ts(tb + kColDk, tb + kColA1 + 32 * (kk >> 1) + 16 + 8 * (kk & 1), nmaj(aq, kk), iKn, 1);
           tc::mma_commit(&sm.g4a);
           tc::mma_commit(&sm.empty[slot_of(kTQ)]);
           tc::mma_commit(&sm.empty[slot_of(kTK)]);
           if (!(ok = wait(&sm.rmw2, par))) break;
           tc::tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
+#pragma unroll kRoll
+          for (int kk = 0; kk < 128 / 16; ++kk)
             tc::mma_bf16_ts(tb + kColA2, tb + kColA1 + 32 * (kk >> 1) + 8 * (kk & 1), nmaj(ao, kk), iVn, 1);
           tc::mma_commit(&sm.g4b);
           tc::mma_commit(&sm.empty[slot_of(kTO)]);
@@ -996,7 +1001,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         tc::mbar_arrive(&sm.f_full);
       }
     }
-  } else if (warp == 3) {
+  } else if (warp == 1) {
     // ------------------------------------------------------------------- dg
     if constexpr (kDg) {
       for (int64_t id = blockIdx.x; id < p.items && ok; id += step) {
@@ -1078,6 +1083,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         const float out_f = p.a.scale * exp_of(hj), in_f = exp_of(gc - hj);  // of the products with S and dS'
         const float eGC = exp_of(gc);
         const float block_f = p.a.scale * exp_of(sm.hi[32 * quarter] - hj);  // of the 32 columns where quarter > q4
+        float kdk = 0.f;  // k . dk, its part from within the chunk
         if (!(ok = warp_wait(&sm.g1, par))) break;
         tc::tc_fence_after();
         // ---- P^T, E^T ------------------------------------------------------
@@ -1100,35 +1106,39 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
               float a2[16];
               tc::tmem_ld16(tl + kColA2 + c0, a2);
               tc::tmem_wait_ld();
-              if (quarter > q4) {
-                const uint64_t* rr = reinterpret_cast<const uint64_t*>(sm.r + c0);
-                const uint64_t bf2 = tc::pack2(block_f, block_f);
+              const float4* src = reinterpret_cast<const float4*>((quarter > q4 ? sm.r : sm.g2) + c0);
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                  const uint64_t f2 = tc::mul2(rr[e / 2], bf2);
-                  tc::unpack2(tc::mul2(tc::pack2(a1[b][e], a1[b][e + 1]), f2), a1[b][e], a1[b][e + 1]);
-                  tc::unpack2(tc::mul2(tc::pack2(a2[e], a2[e + 1]), f2), a2[e], a2[e + 1]);
-                }
-              } else {
-                const float4* gg = reinterpret_cast<const float4*>(sm.g2 + c0);
+              for (int e = 0; e < 4; ++e) {
+                const float4 x = src[e];
+                float f[4] = {x.x, x.y, x.z, x.w};
+                if (quarter > q4) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float4 x = gg[e];
-                  const float y[4] = {x.x, x.y, x.z, x.w};
+                  for (int u = 0; u < 4; ++u) f[u] *= block_f;
+                } else {
 #pragma unroll
-                  for (int u = 0; u < 4; ++u) {  // (a select: what lies in the past may not be finite)
+                  for (int u = 0; u < 4; ++u) {  // (selects: what lies in the past may not be finite)
                     const int i = 4 * e + u;
-                    const float f = p.a.scale * exp2_approx(y[u] - gj);
                     const bool keep = 16 * b + i >= lane;
-                    a1[b][i] = keep ? a1[b][i] * f : 0.f;
-                    a2[i] = keep ? a2[i] * f : 0.f;
+                    f[u] = p.a.scale * exp2_approx(f[u] - gj);
+                    a1[b][i] = keep ? a1[b][i] : 0.f;
+                    a2[i] = keep ? a2[i] : 0.f;
+                    f[u] = keep ? f[u] : 0.f;
                   }
                 }
-              }
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                pp[e] = pack_bf16(a1[b][2 * e], a1[b][2 * e + 1]);
-                ee[e] = pack_bf16(a2[2 * e], a2[2 * e + 1]);
+                for (int u = 0; u < 2; ++u) {
+                  const int i = 4 * e + 2 * u;
+                  const uint64_t f2 = tc::pack2(f[2 * u], f[2 * u + 1]);
+                  float y, z;
+                  tc::unpack2(tc::mul2(tc::pack2(a2[i], a2[i + 1]), f2), y, z);
+                  ee[i / 2] = pack_bf16(y, z);
+                  if constexpr (kDg) {
+                    kdk = fmaf(__uint_as_float(ee[i / 2] << 16), a1[b][i], kdk);
+                    kdk = fmaf(__uint_as_float(ee[i / 2] & 0xffff0000u), a1[b][i + 1], kdk);
+                  }
+                  tc::unpack2(tc::mul2(tc::pack2(a1[b][i], a1[b][i + 1]), f2), y, z);
+                  pp[i / 2] = pack_bf16(y, z);
+                }
               }
             }
             tc::tmem_st8(cs + 8 * b, pp);
@@ -1170,6 +1180,9 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           tc::tmem_st16f(ck, y);
           if constexpr (kDg) kin += dot16(krow, p0 + 2 * b, row, y);
         }
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        tc::mbar_arrive(&sm.rmw1);
         if constexpr (kDg) {  // <S, dS'>: this thread's share of the tiles
           const uint4* s4 = reinterpret_cast<const uint4*>(tile(kTS));
           const uint4* d4 = reinterpret_cast<const uint4*>(tile(kTD));
@@ -1177,13 +1190,11 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           for (int e = tid - 128; e < K * V / 8; e += 512) sdot += dot8(s4[e], d4[e]);
           sdot *= eGC;
         }
-        tc::tmem_wait_st();
-        tc::tc_fence_before();
-        tc::mbar_arrive(&sm.rmw1);
         release(kTS);
         release(kTD);
         release(kTV);
         release(kTO);
+        release(kTK);
         if (!(ok = warp_wait(&sm.g3, par))) break;
         tc::tc_fence_after();
 #pragma unroll 1
@@ -1202,7 +1213,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         // ---- results ---------------------------------------------------------
         if (!(ok = warp_wait(&sm.g4a, par))) break;
         tc::tc_fence_after();
-        float xy = 0.f;
+        float xy = -(kdk + kin);
 #pragma unroll 1
         for (int z = 0; z < 2; ++z) {  // dq, dk
           __nv_bfloat16* out = static_cast<__nv_bfloat16*>(z ? p.gr.dk : p.gr.dq) + (tok * H + w.h) * K + quarter * (K / 4);
@@ -1213,8 +1224,7 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
             tc::tmem_ld16(tl + (z ? kColDk : kColDq) + quarter * (K / 4) + 16 * b, x);
             tc::tmem_wait_ld();
             if constexpr (kDg) {
-              const float d = dot16(z ? krow : qrow, p0 + 2 * b, row, x);
-              xy += z ? -d : d;
+              if (z == 0) xy += dot16(qrow, p0 + 2 * b, row, x);
             }
             if (group > 1) {  // this CTA's running sums over the value heads of the group
               if (j > 0) {
@@ -1232,22 +1242,11 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
             }
             if (inside && j + 1 == group) st_32bytes(out + 16 * b, pack8(x), pack8(x + 8));
           }
-          release(z ? kTK : kTQ);
+          __syncwarp();
+          if (lane + z == 0) tc::mbar_arrive(&sm.empty[slot_of(kTQ)]);
         }
         tc::tc_fence_before();
         tc::mbar_arrive(&sm.qk_free);
-        if (!(ok = warp_wait(&sm.g4b, par))) break;
-        tc::tc_fence_after();
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.gr.dv) + (tok * HV + hv) * V + quarter * (V / 4);
-#pragma unroll 1
-        for (int b = 0; b < V / 64; ++b) {
-          float x[16];
-          tc::tmem_ld16(tl + kColA2 + quarter * (V / 4) + 16 * b, x);
-          tc::tmem_wait_ld();
-          if (inside) st_32bytes(out + 16 * b, pack8(x), pack8(x + 8));
-        }
-        tc::tc_fence_before();
-        tc::mbar_arrive(&sm.dv_free);
         if constexpr (kDg) {
           if (n > 0 && !(ok = warp_wait(&sm.xy_free, (n - 1) & 1))) break;
           atomicAdd(&sm.xy[quarter >> 1][row], xy);
@@ -1262,6 +1261,18 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           }
           tc::mbar_arrive(&sm.xy_full);
         }
+        if (!(ok = warp_wait(&sm.g4b, par))) break;
+        tc::tc_fence_after();
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.gr.dv) + (tok * HV + hv) * V + quarter * (V / 4);
+#pragma unroll 1
+        for (int b = 0; b < V / 64; ++b) {
+          float x[16];
+          tc::tmem_ld16(tl + kColA2 + quarter * (V / 4) + 16 * b, x);
+          tc::tmem_wait_ld();
+          if (inside) st_32bytes(out + 16 * b, pack8(x), pack8(x + 8));
+        }
+        tc::tc_fence_before();
+        tc::mbar_arrive(&sm.dv_free);
       }
     }
   }
