@@ -74,6 +74,7 @@ struct LaSegs {
   int64_t entries;      // segments over all sequences (packed and cut: an upper bound)
   const LaChunk* map;   // [entries] (sequence, segment), packed and cut only
   const int32_t* first; // [N + 1] first entry of each sequence
+  const int32_t* order; // [entries] long entries first, then how many hold `len` chunks; packed only
   float* X;             // [entries, HV, K, V] states, where cut
   float* D;             // [entries, HV] decay over the segment
   GDN2_DEV bool get(int64_t entry, const LaGeom&, int64_t& n, int64_t& s) const {
@@ -82,7 +83,7 @@ struct LaSegs {
       s = map[entry].c;
       return n >= 0;
     }
-    n = entry / per;
+    n = (uint32_t)entry / (uint32_t)per;
     s = entry - n * per;
     return true;
   }
@@ -92,6 +93,7 @@ struct LaSegs {
 struct LaSegWs {
   LaChunk* map;
   int32_t* first;
+  int32_t* order;
   float* X;
   float* D;
 };
@@ -126,8 +128,8 @@ inline int64_t la_num_chunks(const gdn2_linear_attn_args& a) {
 // head, none shorter than 8 chunks (a cut costs a second pass over k and v).
 inline LaSegs la_segs(const gdn2_linear_attn_args& a, const LaSegWs& ws) {
   const int64_t C = kLaChunkTc, NT = la_num_chunks(a), slices = a.HV * (a.V / 64);
-  const int64_t most = a.cu_seqlens ? (a.T + C - 1) / C : (a.T + C - 1) / C;  // chunks of the longest sequence
-  const int64_t want = std::max<int64_t>(1, kLaSms / slices);                 // segments over all sequences
+  const int64_t most = (a.T + C - 1) / C;                      // chunks of the longest sequence
+  const int64_t want = std::max<int64_t>(1, kLaSms / slices);  // segments over all sequences
   LaSegs g{};
   int64_t len = most;
   if (a.cu_seqlens) len = (NT + want - 1) / want;
@@ -137,6 +139,7 @@ inline LaSegs la_segs(const gdn2_linear_attn_args& a, const LaSegWs& ws) {
   g.len = (int)(g.multi ? len : std::max<int64_t>(most, 1));
   g.per = g.multi ? (most + len - 1) / len : 1;
   g.entries = a.cu_seqlens ? (g.multi ? a.T / (C * len) + a.N : a.N) : a.N * g.per;
+  g.order = ws.order;
   if (g.multi) {
     g.map = a.cu_seqlens ? ws.map : nullptr;
     g.first = ws.first;
@@ -165,6 +168,7 @@ inline size_t la_ws_layout(const gdn2_linear_attn_args& a, void* base, LaWs* out
   }
   if (la_tc(a)) {
     const LaSegs g = la_segs(a, w.seg);
+    if (a.cu_seqlens) w.seg.order = (int32_t*)take(((size_t)g.entries + 1) * 4);
     if (g.multi) {
       if (a.cu_seqlens) {
         w.seg.map = (LaChunk*)take((size_t)g.entries * sizeof(LaChunk));

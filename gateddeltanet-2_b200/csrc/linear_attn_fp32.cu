@@ -475,9 +475,9 @@ __global__ void __launch_bounds__(256) la_head_sum_kernel(const float* dg, int64
 }
 
 // (sequence, chunk) of every chunk id of a packed batch, and each sequence's
-// first chunk; the same for segments, of which an empty sequence has one.  One CTA walks the lengths 1024 at a time with a block prefix sum.
-__global__ void __launch_bounds__(1024) la_chunk_map_kernel(LaGeom geo, int64_t unit, int64_t least, LaChunk* map,
-                                                            int32_t* first, int64_t NT) {
+// first chunk; the same for segments, of which an empty sequence has one.  One
+// CTA walks the lengths 1024 at a time with a block prefix sum.
+GDN2_DEV void chunk_map(const LaGeom& geo, int64_t unit, int64_t least, LaChunk* map, int32_t* first, int64_t NT) {
   __shared__ int64_t warp_sum[32];
   __shared__ int64_t carry;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -520,6 +520,42 @@ __global__ void __launch_bounds__(1024) la_chunk_map_kernel(LaGeom geo, int64_t 
     }
     map[id] = m;
   }
+  __syncthreads();
+}
+
+// The entries of a scan, long ones first (a counting sort over 1024 classes of
+// lengths; the order within one is of no consequence), so that the CTAs' turns
+// through them add up to nearly the same; after them, how many are full.
+GDN2_DEV void order_entries(const LaGeom& geo, const LaSegs& seg, int32_t* order) {
+  __shared__ int32_t count[1024];
+  __shared__ int32_t warp_sum[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto cls = [&](int64_t e) -> int {
+    int64_t n, s, bos, len, chunks = 0;
+    if (seg.get(e, geo, n, s)) {
+      geo.seq(n, bos, len);
+      chunks = max((len + geo.C - 1) / geo.C - s * seg.len, (int64_t)0);
+    }
+    return chunks >= seg.len ? 0 : 1 + (int)((seg.len - 1 - chunks) * 1022 / max(seg.len - 1, 1));
+  };
+  count[tid] = 0;
+  __syncthreads();
+  for (int64_t e = tid; e < seg.entries; e += 1024) atomicAdd(&count[cls(e)], 1);
+  __syncthreads();
+  const int32_t mine = count[tid];
+  int32_t s = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t y = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += y;
+  }
+  if (lane == 31) warp_sum[warp] = s;
+  __syncthreads();
+  for (int i = 0; i < warp; ++i) s += warp_sum[i];
+  count[tid] = s - mine;
+  if (tid == 0) order[seg.entries] = mine;
+  __syncthreads();
+  for (int64_t e = tid; e < seg.entries; e += 1024) order[atomicAdd(&count[cls(e)], 1)] = (int32_t)e;
 }
 
 // Rows of packed tensors that lie in no sequence (before the first offset,
@@ -528,7 +564,7 @@ struct LaRows {
   void* p[4];
   int64_t bytes[4];  // of one row
 };
-__global__ void __launch_bounds__(256) la_zero_outside_kernel(LaRows r, LaGeom geo) {
+GDN2_DEV void zero_outside(const LaRows& r, const LaGeom& geo, int64_t thread, int64_t threads) {
   int64_t b0, l0, b1, l1;
   geo.seq(0, b0, l0);
   geo.seq(geo.N - 1, b1, l1);
@@ -537,11 +573,34 @@ __global__ void __launch_bounds__(256) la_zero_outside_kernel(LaRows r, LaGeom g
   for (int i = 0; i < 4; ++i) {
     if (!r.p[i]) continue;
     const int64_t units = r.bytes[i] / 2;  // every row is a whole number of 2-byte units
-    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < rows * units; x += (int64_t)gridDim.x * 256) {
+    for (int64_t x = thread; x < rows * units; x += threads) {
       const int64_t k = x / units, row = k < b0 ? k : end + (k - b0);
       static_cast<uint16_t*>(r.p[i])[row * units + x % units] = 0;
     }
   }
+}
+
+// What a packed batch needs before its forward pass: CTA 0 lays out chunks and
+// segments, the others clear rows.  (One launch: they are a few microseconds each.)
+struct LaPacked {
+  LaGeom geo;
+  LaSegs seg;
+  LaRows rows;
+  LaChunk *map, *seg_map;  // or NULL
+  int32_t *first, *seg_first, *order;
+  int64_t NT;
+};
+__global__ void __launch_bounds__(1024) la_packed_kernel(LaPacked p) {
+  if (blockIdx.x > 0) {
+    zero_outside(p.rows, p.geo, (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
+    return;
+  }
+  if (p.map) chunk_map(p.geo, p.geo.C, 0, p.map, p.first, p.NT);
+  if (p.seg_map) chunk_map(p.geo, (int64_t)p.geo.C * p.seg.len, 1, p.seg_map, p.seg_first, p.seg.entries);
+  if (p.order) order_entries(p.geo, p.seg, p.order);
+}
+__global__ void __launch_bounds__(256) la_zero_outside_kernel(LaRows r, LaGeom geo) {
+  zero_outside(r, geo, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
 template <typename T, int K, int V>
@@ -632,20 +691,16 @@ int la_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s
   const LaGeom geo = la_geom(a, ws);
   const bool any = a.B * a.T > 0;
   if (a.cu_seqlens) {
-    if (ws.map) {
-      la_chunk_map_kernel<<<1, 1024, 0, s>>>(geo, geo.C, 0, ws.map, ws.first, la_num_chunks(a));
-      GDN2_LAUNCH_CHECK();
+    const int64_t e = a.dtype == GDN2_BF16 ? 2 : 4;
+    LaPacked p{geo, {}, {{any ? a.o : nullptr}, {a.HV * a.V * e}}, ws.map, nullptr, ws.first, nullptr, nullptr, la_num_chunks(a)};
+    if (la_tc(a)) {
+      p.seg = la_segs(a, ws.seg);
+      p.seg_map = ws.seg.map;
+      p.seg_first = ws.seg.first;
+      p.order = ws.seg.order;
     }
-    if (ws.seg.map) {
-      const LaSegs seg = la_segs(a, ws.seg);
-      la_chunk_map_kernel<<<1, 1024, 0, s>>>(geo, (int64_t)geo.C * seg.len, 1, ws.seg.map, ws.seg.first, seg.entries);
-      GDN2_LAUNCH_CHECK();
-    }
-    if (any) {
-      const int64_t e = a.dtype == GDN2_BF16 ? 2 : 4;
-      la_zero_outside_kernel<<<32, 256, 0, s>>>(LaRows{{a.o}, {a.HV * a.V * e}}, geo);
-      GDN2_LAUNCH_CHECK();
-    }
+    la_packed_kernel<<<33, 1024, 0, s>>>(p);
+    GDN2_LAUNCH_CHECK();
   }
   if (!any) {  // no tokens: the final states are the initial ones
     if (!(a.flags & GDN2_STORE_FINAL)) return 0;

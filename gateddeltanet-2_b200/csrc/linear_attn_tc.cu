@@ -84,6 +84,7 @@ struct ScanArgs {
   LaGeom geo;
   LaSegs seg;
   int64_t tasks;
+  int group;             // value heads per key head
   int pre;               // 1: the pass that only takes segments' own states to X and their decays to D
   const float* init;     // h0 / dht, or NULL
   float* fin;            // ht / dh0, or NULL
@@ -97,11 +98,15 @@ struct Task {
 
 template <bool kBack>
 GDN2_DEV bool find_task(const ScanArgs& p, int64_t id, Task& t) {
-  const uint32_t vs = (uint32_t)(p.a.V >> 6), HV = (uint32_t)p.a.HV, r = (uint32_t)id / vs;
-  t.z = (int)((uint32_t)id % vs);
-  t.hv = r % HV;
+  // the CTAs' turns go back and forth through the tasks, whose lengths fall where they are ordered
+  const uint32_t turn = (uint32_t)id / kLaSms;
+  if (!p.pre && (turn & 1) && (int64_t)(turn + 1) * kLaSms <= p.tasks) id = (int64_t)(2 * turn + 1) * kLaSms - 1 - id;
+  const uint32_t two = (uint32_t)(p.a.V >> 7), HV = (uint32_t)p.a.HV, r = (uint32_t)id >> two;  // 64-column slices: 1 or 2
+  t.z = (int)((uint32_t)id & two);
   t.entry = r / HV;
-  t.h = (uint32_t)t.hv / (HV / (uint32_t)p.a.H);
+  t.hv = r - (uint32_t)t.entry * HV;
+  if (p.seg.order) t.entry = p.seg.order[t.entry];
+  t.h = (uint32_t)t.hv / (uint32_t)p.group;
   int64_t s;
   if (!p.seg.get(t.entry, p.geo, t.n, s)) return false;
   p.geo.seq(t.n, t.bos, t.len);
@@ -156,6 +161,24 @@ GDN2_DEV void st_32bytes(void* p, const uint4& a, const uint4& b) {
     static_cast<uint4*>(p)[0] = a;
     static_cast<uint4*>(p)[1] = b;
   }
+}
+GDN2_DEV void ld_32bytes(const float* p, float* x) {
+  uint32_t r[8];
+  if ((reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(p[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(r[e]);
+}
+// (16-byte aligned, a multiple of 16 bytes)
+GDN2_DEV void prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 // Bounded waits.  One lane: the retry loop is one copy of code.  A whole warp:
 // votes keep it converged in a way that the compiler can see (a call would not).
@@ -228,9 +251,13 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
   // the token coordinate and batch of chunk c in the tensor maps
   auto tok = [&](int c) { return (int)((p.geo.cu ? t.bos : 0) + (int64_t)c * kC); };
   const int64_t step = gridDim.x;
+  int64_t tasks = p.tasks;
+  if constexpr (!kOut) {  // only segments that are full have one after them
+    if (p.pre && p.seg.order) tasks = uniform(min(tasks, (int64_t)p.seg.order[p.seg.entries] * p.a.HV * (p.a.V >> 6)));
+  }
   auto count_chunks = [&]() {  // over all tasks
     uint32_t n = 0;
-    for (int64_t id = blockIdx.x; id < p.tasks; id += step)
+    for (int64_t id = blockIdx.x; id < tasks; id += step)
       if (find_task<kBack>(p, id, t)) n += (uint32_t)max(t.ce - t.cb, 0);
     return n;
   };
@@ -305,9 +332,11 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       tc::prefetch_tensormap(&tmX);
       tc::prefetch_tensormap(&tmY);
       if (kOut) tc::prefetch_tensormap(&tmQ);
-      for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
+      for (int64_t id = blockIdx.x; id < tasks && ok; id += step) {
         if (!find_task<kBack>(p, id, t)) continue;
         const int b = p.geo.cu ? 0 : (int)t.n;
+        if (t.head && p.init && t.z == 0)  // both slices' state, ahead of the task's turn
+          prefetch_l2(p.init + (t.n * p.a.HV + t.hv) * K * p.a.V, (uint32_t)(K * p.a.V * 4));
         for (int i = 0; i < t.ce - t.cb; ++i, ++it) {
           const uint32_t sx = it % NX, sy = it % NY;
           const int tt = tok(nth(i));
@@ -336,7 +365,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
     // ---------------------- MMAs: Q K^T, P V; without outputs: entering states out
     if constexpr (!kOut) {
       if (kStore && lane == 0) {
-        for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
+        for (int64_t id = blockIdx.x; id < tasks && ok; id += step) {
           if (!find_task<kBack>(p, id, t)) continue;
           for (int i = 0; i < t.ce - t.cb; ++i, ++it) {
             if (!(ok = wait(&sm.s_full, it & 1))) break;
@@ -428,7 +457,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       __syncwarp();
       return true;
     };
-    for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
+    for (int64_t id = blockIdx.x; id < tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
       // this lane's four tokens of a chunk lie `gs` bytes apart (0: one decay for all)
       const int es = p.dec.dtype == GDN2_BF16 ? 2 : 4;
@@ -493,7 +522,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
   } else if (kOut && warp < 12) {
     // --------------------------------------------------------------- scores
     const int w = warp & 3, i = 32 * w + lane, p2 = (warp - 4) >> 2;  // columns 64 p2 .. 64 p2 + 63
-    for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
+    for (int64_t id = blockIdx.x; id < tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
       for (int j = 0; j < t.ce - t.cb; ++j, ++it) {
         const int s = it & 1;
@@ -599,16 +628,17 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       return true;
     };
     const int64_t KV = (int64_t)K * p.a.V;
-    for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
+    for (int64_t id = blockIdx.x; id < tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
       const int64_t at = (int64_t)row * p.a.V + 64 * t.z;
       const float* src = t.head ? (p.init ? p.init + (t.n * p.a.HV + t.hv) * KV : nullptr)
                          : p.pre ? nullptr
                                  : p.seg.X + ((t.entry + (kBack ? 1 : -1)) * p.a.HV + t.hv) * KV;
 #pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        const float4 x = src ? *reinterpret_cast<const float4*>(src + at + 4 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
-        st[4 * q] = x.x; st[4 * q + 1] = x.y; st[4 * q + 2] = x.z; st[4 * q + 3] = x.w;
+      for (int q = 0; q < 64; ++q) st[q] = 0.f;
+      if (src) {
+#pragma unroll
+        for (int q = 0; q < 64; q += 8) ld_32bytes(src + at + q, st + q);
       }
       const int nloc = t.ce - t.cb;
       for (int i = 0; i <= nloc; ++i) {
@@ -671,7 +701,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       tc::mbar_arrive(&sm.o_free);
       return true;
     };
-    for (int64_t id = blockIdx.x; id < p.tasks && ok; id += step) {
+    for (int64_t id = blockIdx.x; id < tasks && ok; id += step) {
       if (!get_task<kBack>(p, id, t)) continue;
       __nv_bfloat16* const row0 =
           static_cast<__nv_bfloat16*>(p.a.o) + ((t.bos + i) * p.a.HV + t.hv) * p.a.V + 64 * t.z;
@@ -702,21 +732,22 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
 template <bool kBack>
 __global__ void __launch_bounds__(128) la_segment_kernel(LaSegs seg, LaGeom geo, int64_t HV, int64_t KV) {
   const int64_t n = blockIdx.x / HV, hv = blockIdx.x % HV;
-  const int64_t e = ((int64_t)blockIdx.y * 128 + threadIdx.x) * 4;
   int64_t bos, len;
   geo.seq(n, bos, len);
   const int64_t nch = (len + kC - 1) / kC, ns = nch > 0 ? (nch + seg.len - 1) / seg.len : 1;
   const int64_t e0 = seg.first_of(n);
-  if (e >= KV || ns < 3) return;  // the first segment's term is a whole state already, the last one's is not used
-  auto at = [&](int64_t s) {
-    return reinterpret_cast<float4*>(seg.X + ((e0 + (kBack ? ns - 1 - s : s)) * HV + hv) * KV + e);
-  };
-  float4 x = *at(0);
-  for (int64_t s = 1; s < ns - 1; ++s) {
-    const float f = seg.D[(e0 + (kBack ? ns - 1 - s : s)) * HV + hv];
-    float4 y = *at(s);
-    x = make_float4(fmaf(f, x.x, y.x), fmaf(f, x.y, y.y), fmaf(f, x.z, y.z), fmaf(f, x.w, y.w));
-    *at(s) = x;
+  if (ns < 3) return;  // the first segment's term is a whole state already, the last one's is not used
+  for (int64_t e = ((int64_t)blockIdx.y * 128 + threadIdx.x) * 4; e < KV; e += (int64_t)gridDim.y * 512) {
+    auto at = [&](int64_t s) {
+      return reinterpret_cast<float4*>(seg.X + ((e0 + (kBack ? ns - 1 - s : s)) * HV + hv) * KV + e);
+    };
+    float4 x = *at(0);
+    for (int64_t s = 1; s < ns - 1; ++s) {
+      const float f = seg.D[(e0 + (kBack ? ns - 1 - s : s)) * HV + hv];
+      float4 y = *at(s);
+      x = make_float4(fmaf(f, x.x, y.x), fmaf(f, x.y, y.y), fmaf(f, x.z, y.z), fmaf(f, x.w, y.w));
+      *at(s) = x;
+    }
   }
 }
 
@@ -1359,8 +1390,8 @@ int scan(ScanArgs& p, const ScanMaps& m, bool store, cudaStream_t s) {
     p.pre = 1;
     if (int st = run_scan<K, false, false, kBack>(p, m, s)) return st;
     const int64_t KV = p.a.K * p.a.V;
-    la_segment_kernel<kBack><<<dim3((unsigned)(p.a.N * p.a.HV), (unsigned)((KV + 511) / 512)), 128, 0, s>>>(
-        p.seg, p.geo, p.a.HV, KV);
+    const int64_t states = p.a.N * p.a.HV, parts = std::min((KV + 511) / 512, std::max<int64_t>(1, 16 * kLaSms / states));
+    la_segment_kernel<kBack><<<dim3((unsigned)states, (unsigned)parts), 128, 0, s>>>(p.seg, p.geo, p.a.HV, KV);
     GDN2_LAUNCH_CHECK();
     p.pre = 0;
   }
@@ -1371,7 +1402,7 @@ int scan(ScanArgs& p, const ScanMaps& m, bool store, cudaStream_t s) {
 }  // namespace
 
 int la_tc_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
-  ScanArgs p{a, la_decay(a), la_geom(a, ws), la_segs(a, ws.seg), 0, 0, (a.flags & GDN2_HAS_H0) ? a.h0 : nullptr,
+  ScanArgs p{a, la_decay(a), la_geom(a, ws), la_segs(a, ws.seg), 0, (int)(a.HV / a.H), 0, (a.flags & GDN2_HAS_H0) ? a.h0 : nullptr,
              (a.flags & GDN2_STORE_FINAL) ? a.ht : nullptr};
   p.tasks = p.seg.entries * a.HV * (a.V / 64);
   if (p.tasks >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
@@ -1408,8 +1439,9 @@ int bwd(const BwdArgs& p, const CUtensorMap (&m)[6], cudaStream_t s) {
 
 int la_tc_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
                      const LaBwdWs& bw, cudaStream_t s) {
-  ScanArgs sc{a, la_decay(a), la_geom(a, ws), la_segs(a, bw.seg), 0, 0, gr.dht, gr.dh0};
-  if (sc.seg.cut) {  // the forward's map of the cut
+  ScanArgs sc{a, la_decay(a), la_geom(a, ws), la_segs(a, bw.seg), 0, (int)(a.HV / a.H), 0, gr.dht, gr.dh0};
+  sc.seg.order = ws.seg.order;  // the forward's
+  if (sc.seg.cut) {
     sc.seg.map = ws.seg.map;
     sc.seg.first = ws.seg.first;
   }
