@@ -252,7 +252,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
   auto tok = [&](int c) { return (int)((p.geo.cu ? t.bos : 0) + (int64_t)c * kC); };
   const int64_t step = gridDim.x;
   int64_t tasks = p.tasks;
-  if constexpr (!kOut) {  // only segments that are full have one after them
+  if constexpr (!kOut && !kBack) {  // only segments that are full have one after them
     if (p.pre && p.seg.order) tasks = uniform(min(tasks, (int64_t)p.seg.order[p.seg.entries] * p.a.HV * (p.a.V >> 6)));
   }
   auto count_chunks = [&]() {  // over all tasks

@@ -148,6 +148,15 @@ def test_packed(gdn2, lens, h0, dtype):
     check(*run_both(gdn2, d, lens=lens), d, dtype)
 
 
+@pytest.mark.parametrize("lens", [
+    [40, 1, 0, 129, 1310, 3, 128, 256, 64, 17, 300, 0, 5, 127, 2, 90, 33, 1, 200, 11, 130, 7, 65, 18],  # one is cut
+    [130, 1, 0, 200, 90] * 8])  # none is
+def test_packed_more_work_than_one_turn(gdn2, lens):
+    """More segments and heads than CTAs, of unlike lengths."""
+    d = make(31, 1, sum(lens), 4, 8, 64, 64, torch.bfloat16, "token", h0=True, N=len(lens))
+    check(*run_both(gdn2, d, lens=lens), d, torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strong_decays_and_resets(gdn2, dtype):
     """Decays down to e^-40 a token, and -inf: the state is forgotten, later tokens keep full precision."""
