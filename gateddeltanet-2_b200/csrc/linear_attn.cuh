@@ -125,7 +125,11 @@ inline int64_t la_num_chunks(const gdn2_linear_attn_args& a) {
 }
 
 // The cut of the scans: enough segments for one per SM and 64-column slice of a
-// head, none shorter than 8 chunks (a cut costs a second pass over k and v).
+// head, none shorter than 4 chunks.  A cut costs a second pass over k and v and two
+// launches, so it has to take two segments and 8 chunks off the walk.  One sequence,
+// 16 heads, K = V = 128, uncut and cut: 1024 tokens 22 and 30 us (2 x 4 chunks: not
+// cut), 2048 tokens 37 and 33 us (4 x 4; 2 x 8: 41 us), 16384 tokens 261 and 121 us;
+// one head, 16384 tokens: 243 us, and 44 or 39 us with at least 8 or 4 chunks.
 inline LaSegs la_segs(const gdn2_linear_attn_args& a, const LaSegWs& ws) {
   const int64_t C = kLaChunkTc, NT = la_num_chunks(a), slices = a.HV * (a.V / 64);
   const int64_t most = (a.T + C - 1) / C;                      // chunks of the longest sequence
@@ -134,8 +138,8 @@ inline LaSegs la_segs(const gdn2_linear_attn_args& a, const LaSegWs& ws) {
   int64_t len = most;
   if (a.cu_seqlens) len = (NT + want - 1) / want;
   else if (a.N < want) len = (most + want / std::max<int64_t>(a.N, 1) - 1) / (want / std::max<int64_t>(a.N, 1));
-  len = std::max<int64_t>(len, 8);
-  g.multi = len < most;
+  len = std::max<int64_t>(len, 4);
+  g.multi = most >= 2 * len + 8;
   g.len = (int)(g.multi ? len : std::max<int64_t>(most, 1));
   g.per = g.multi ? (most + len - 1) / len : 1;
   g.entries = a.cu_seqlens ? (g.multi ? a.T / (C * len) + a.N : a.N) : a.N * g.per;

@@ -6,7 +6,10 @@
 // columns in K / (threads / (VT / 4)) rows; all its loads are issued before
 // anything waits on them.  o needs one reduction over the rows: each thread's
 // own rows, the lanes of its warp that share its columns, then the warps
-// through shared memory.
+// through shared memory.  Tiles are 64 columns wide: 32 floats of state a thread
+// at K = 128, four CTAs an SM.
+// Bound by bandwidth: 256 sequences of 16 heads, K = V = 128 (541 MB) take 88 us,
+// 6.15 TB/s; four sequences 8 us, which is the launch and one trip to memory and back.
 #include "linear_attn.cuh"
 #include "profile.cuh"
 
