@@ -35,7 +35,7 @@
 // Q K^T once per 64 columns.
 // What bounds it: a chunk's products keep the tensor pipe busy for some 2050 clocks
 // and read their operands from shared memory for some 2950 (K = 128); the roles'
-// hand-overs bring that to 3300 to 3500.  Measured at 16 heads, K = V = 128:
+// hand-overs bring that to 3400 (batches in L2) to 4300.  Measured at 16 heads, K = V = 128:
 // 4 sequences of 4096 tokens 76 us (268 MB, 3.5 TB/s; 83 us where the states are kept
 // for the backward, 48 us for the reverse scan without outputs); 65536 tokens 277 us
 // after 138 us for the segments' own states; 23 packed sequences of 9001 tokens 74 us.
