@@ -13,6 +13,11 @@
 // a running sum of those over the chunks of a sequence, and every chunk's
 // outputs.  Running sums of g and their differences are held in fp64: their
 // exponentials then carry only their own rounding, however long or strong the decay.
+// Bound by shared memory and the fp32 pipes: a product of 64 x 64 x 64 takes 16 FMAs
+// a step of k in each of 256 threads, for 3 to 5 wavefronts of operands; 64 tokens a
+// chunk keep six tiles of the backward in one SM.  Measured, both directions: 2 x 1000
+// tokens, 4 heads of 64 (128 CTAs of one wave) 75 us in six launches, 4 x 4096 tokens,
+// 16 heads of 128, 3.3 ms; with operands loaded word by word 107 us and 5.0 ms.
 #include "linear_attn.cuh"
 #include "profile.cuh"
 
@@ -21,28 +26,44 @@ namespace {
 
 constexpr int kC = kLaChunkF32;
 constexpr int kThreads = 256;
-constexpr int kLdP = kC + 1;
+constexpr int kPad = 4;  // rows of tiles stay on 16 bytes, and 8 of them start in 8 groups of banks
+constexpr int kLdP = kC + kPad;
 
-// acc[r][c] += sum_k A(4 ty + r, k) B(k, tx + 16 c); strides in elements.
-// A row is shared by the 16 threads of a half warp (broadcast); consecutive tx
-// read consecutive columns, or rows of odd length (no bank conflicts either way).
-template <int NJ>
-GDN2_DEV void tile_mm(float (&acc)[4][NJ], const float* A, int sai, int sak, const float* B, int sbk, int sbj,
-                      int kdim) {
+// acc[r][c] += sum_k A(4 ty + r, k) B(k, tx + 16 c), four k at a time.  kAt: A is
+// stored k by rows (row k holds all i), else i by rows; kBt: B is stored column by
+// column (row j holds all k), else k by rows.  What lies along a row is loaded 16 bytes at a
+// time: 3 or 5 shared-memory wavefronts a step of k instead of 8 of single words.
+template <bool kAt, bool kBt, int NJ>
+GDN2_DEV void tile_mm(float (&acc)[4][NJ], const float* A, int lda, const float* B, int ldb, int kdim) {
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  A += 4 * ty * sai;
-  B += tx * sbj;
-#pragma unroll 4
-  for (int k = 0; k < kdim; ++k) {
-    float x[4], y[NJ];
+  A += kAt ? 4 * ty : 4 * ty * lda;
+  B += kBt ? tx * ldb : tx;
+#pragma unroll 2
+  for (int k = 0; k < kdim; k += 4) {
+    float x[4][4], y[NJ][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = A[r * sai + k * sak];
+    for (int u = 0; u < 4; ++u) {
+      const float4 v = *reinterpret_cast<const float4*>(kAt ? A + (k + u) * lda : A + u * lda + k);
+      const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int c = 0; c < NJ; ++c) y[c] = B[k * sbk + 16 * c * sbj];
+      for (int e = 0; e < 4; ++e) (kAt ? x[e][u] : x[u][e]) = w[e];
+    }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int c = 0; c < NJ; ++c) {
+      if constexpr (kBt) {
+        const float4 v = *reinterpret_cast<const float4*>(B + 16 * c * ldb + k);
+        y[c][0] = v.x; y[c][1] = v.y; y[c][2] = v.z; y[c][3] = v.w;
+      } else {
 #pragma unroll
-      for (int c = 0; c < NJ; ++c) acc[r][c] = fmaf(x[r], y[c], acc[r][c]);
+        for (int u = 0; u < 4; ++u) y[c][u] = B[(k + u) * ldb + 16 * c];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < NJ; ++c) acc[r][c] = fmaf(x[r][u], y[c][u], acc[r][c]);
   }
 }
 
@@ -54,12 +75,36 @@ GDN2_DEV void zero(float (&acc)[4][NJ]) {
     for (int c = 0; c < NJ; ++c) acc[r][c] = 0.f;
 }
 
-// L rows of D elements (row stride st) into a padded fp32 tile, zero rows after them
-template <typename T, int D>
-GDN2_DEV void load_rows(float* dst, const T* src, int64_t st, int L) {
-  for (int i = threadIdx.x; i < kC * D; i += kThreads) {
-    const int r = i / D, c = i % D;
-    dst[r * (D + 1) + c] = r < L ? to_f(src[r * st + c]) : 0.f;
+// L rows of D elements (row stride st, 16-byte steps) into a padded tile, zero rows after them; all loads at once
+template <int D>
+GDN2_DEV void load_rows(float* dst, const float* src, int64_t st, int L) {
+  constexpr int kEach = kC * D / 4 / kThreads;
+  float4 x[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x + e * kThreads, r = i / (D / 4), c = i % (D / 4) * 4;
+    x[e] = r < L ? *reinterpret_cast<const float4*>(src + r * st + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x + e * kThreads, r = i / (D / 4), c = i % (D / 4) * 4;
+    *reinterpret_cast<float4*>(dst + r * (D + kPad) + c) = x[e];
+  }
+}
+// ROWS rows of 64 or more columns of a state with V columns
+template <int ROWS, int COLS>
+GDN2_DEV void load_state(float* dst, const float* src, int V) {
+  constexpr int kEach = ROWS * COLS / 4 / kThreads;
+  float4 x[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x + e * kThreads, r = i / (COLS / 4), c = i % (COLS / 4) * 4;
+    x[e] = *reinterpret_cast<const float4*>(src + (int64_t)r * V + c);
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = threadIdx.x + e * kThreads, r = i / (COLS / 4), c = i % (COLS / 4) * 4;
+    *reinterpret_cast<float4*>(dst + r * (COLS + kPad) + c) = x[e];
   }
 }
 
@@ -100,28 +145,27 @@ GDN2_DEV bool locate(const LaGeom& geo, int64_t id, Where& w) {
 // One chunk's own term of the state recurrence, sum_t w_t x_t y_t^T: forward
 // x = k, y = v, w_t = e^{G_C - G_t}; backward x = q, y = do, w_t = scale e^{G_t}.
 // 8 x 8 (or smaller) outputs per thread.
-template <typename T, int K, int V, bool kBack>
-__global__ void __launch_bounds__(kThreads) la_state_kernel(const T* x, int64_t xb, int64_t xt, int64_t xh, const T* y,
+template <int K, int V, bool kBack>
+__global__ void __launch_bounds__(kThreads) la_state_kernel(const float* x, int64_t xb, int64_t xt, int64_t xh, const float* y,
                                                             int64_t yb, int64_t yt, int64_t yh, LaDecay dec,
                                                             LaGeom geo, int HV, int group, float scale, float* states,
                                                             float* total) {
-  extern __shared__ float sm[];
+  extern __shared__ __align__(16) float sm[];
   float* X = sm;
-  float* Y = X + kC * (K + 1);
+  float* Y = X + kC * (K + kPad);
   __shared__ double G[kC];
+  __shared__ float weight[kC];
   Where w;
   const int hv = blockIdx.y;
   if (!locate(geo, blockIdx.x, w)) return;
-  load_rows<T, K>(X, x + w.b * xb + w.t0 * xt + (hv / group) * xh, xt, w.L);
-  load_rows<T, V>(Y, y + w.b * yb + w.t0 * yt + hv * yh, yt, w.L);
+  load_rows<K>(X, x + w.b * xb + w.t0 * xt + (hv / group) * xh, xt, w.L);
+  load_rows<V>(Y, y + w.b * yb + w.t0 * yt + hv * yh, yt, w.L);
   chunk_sums(G, dec, w.b, w.t0, hv, w.L);
   __syncthreads();
   if (threadIdx.x == 0 && total) total[(int64_t)blockIdx.x * HV + hv] = expf((float)G[kC - 1]);
-  for (int i = threadIdx.x; i < kC * V; i += kThreads) {
-    const int t = i / V;
-    const float f = kBack ? scale * expf((float)G[t]) : expf((float)(G[kC - 1] - G[t]));
-    if (t < w.L) Y[t * (V + 1) + i % V] *= f;
-  }
+  if (threadIdx.x < kC)
+    weight[threadIdx.x] =
+        kBack ? scale * expf((float)G[threadIdx.x]) : expf((float)(G[kC - 1] - G[threadIdx.x]));
   __syncthreads();
   constexpr int R = K / 16, NJ = V / 16;
   float acc[R][NJ];
@@ -130,12 +174,17 @@ __global__ void __launch_bounds__(kThreads) la_state_kernel(const T* x, int64_t 
 #pragma unroll
     for (int c = 0; c < NJ; ++c) acc[r][c] = 0.f;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll 4
   for (int t = 0; t < w.L; ++t) {
     float a[R], bb[NJ];
 #pragma unroll
-    for (int r = 0; r < R; ++r) a[r] = X[t * (K + 1) + ty + 16 * r];
+    for (int r = 0; r < R; r += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(X + t * (K + kPad) + R * ty + r);
+      a[r] = x.x; a[r + 1] = x.y; a[r + 2] = x.z; a[r + 3] = x.w;
+    }
+    const float f = weight[t];
 #pragma unroll
-    for (int c = 0; c < NJ; ++c) bb[c] = Y[t * (V + 1) + tx + 16 * c];
+    for (int c = 0; c < NJ; ++c) bb[c] = f * Y[t * (V + kPad) + tx + 16 * c];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -145,7 +194,7 @@ __global__ void __launch_bounds__(kThreads) la_state_kernel(const T* x, int64_t 
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int c = 0; c < NJ; ++c) dst[(ty + 16 * r) * V + tx + 16 * c] = acc[r][c];
+    for (int c = 0; c < NJ; ++c) dst[(R * ty + r) * V + tx + 16 * c] = acc[r][c];
 }
 
 // The running sum over a sequence's chunks, in place: states[c] becomes the
@@ -186,24 +235,24 @@ __global__ void __launch_bounds__(128) la_prefix_kernel(float* states, const flo
   if (fin) *reinterpret_cast<float4*>(fin + nh * KV + e) = s;
 }
 
-template <typename T, int K, int V>
+template <int K, int V>
 __global__ void __launch_bounds__(kThreads) la_out_kernel(gdn2_linear_attn_args a, LaDecay dec, LaGeom geo,
                                                           const float* states) {
-  extern __shared__ float sm[];
+  extern __shared__ __align__(16) float sm[];
   float* Q = sm;
-  float* Kt = Q + kC * (K + 1);
-  float* Vt = Kt + kC * (K + 1);
-  float* P = Vt + kC * (V + 1);
+  float* Kt = Q + kC * (K + kPad);
+  float* Vt = Kt + kC * (K + kPad);
+  float* P = Vt + kC * (V + kPad);
   float* S = P + kC * kLdP;  // 64 rows of the state at a time
   __shared__ double G[kC];
   Where w;
   const int64_t HV = a.HV, hv = blockIdx.y, h = hv / (HV / a.H);
   if (!locate(geo, blockIdx.x, w)) return;
-  load_rows<T, K>(Q, static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.t0 * a.q_stride[1] + h * a.q_stride[2],
+  load_rows<K>(Q, static_cast<const float*>(a.q) + w.b * a.q_stride[0] + w.t0 * a.q_stride[1] + h * a.q_stride[2],
                   a.q_stride[1], w.L);
-  load_rows<T, K>(Kt, static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.t0 * a.k_stride[1] + h * a.k_stride[2],
+  load_rows<K>(Kt, static_cast<const float*>(a.k) + w.b * a.k_stride[0] + w.t0 * a.k_stride[1] + h * a.k_stride[2],
                   a.k_stride[1], w.L);
-  load_rows<T, V>(Vt, static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.t0 * a.v_stride[1] + hv * a.v_stride[2],
+  load_rows<V>(Vt, static_cast<const float*>(a.v) + w.b * a.v_stride[0] + w.t0 * a.v_stride[1] + hv * a.v_stride[2],
                   a.v_stride[1], w.L);
   chunk_sums(G, dec, w.b, w.t0, hv, w.L);
   __syncthreads();
@@ -211,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) la_out_kernel(gdn2_linear_attn_args 
   {
     float p[4][4];
     zero(p);
-    tile_mm(p, Q, K + 1, 1, Kt, 1, K + 1, K);
+    tile_mm<false, true>(p, Q, K + kPad, Kt, K + kPad, K);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -226,9 +275,9 @@ __global__ void __launch_bounds__(kThreads) la_out_kernel(gdn2_linear_attn_args 
   const float* st = states + ((int64_t)blockIdx.x * HV + hv) * K * V;
   for (int k0 = 0; k0 < K; k0 += 64) {
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * V; i += kThreads) S[(i / V) * (V + 1) + i % V] = st[k0 * V + i];
+    load_state<64, V>(S, st + k0 * V, V);
     __syncthreads();
-    tile_mm(o, Q + k0, K + 1, 1, S, V + 1, 1, 64);
+    tile_mm<false, false>(o, Q + k0, K + kPad, S, V + kPad, 64);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -236,14 +285,14 @@ __global__ void __launch_bounds__(kThreads) la_out_kernel(gdn2_linear_attn_args 
 #pragma unroll
     for (int c = 0; c < NJ; ++c) o[r][c] *= f;
   }
-  tile_mm(o, P, kLdP, 1, Vt, V + 1, 1, kC);
-  T* out = static_cast<T*>(a.o);
+  tile_mm<false, false>(o, P, kLdP, Vt, V + kPad, kC);
+  float* out = static_cast<float*>(a.o);
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int c = 0; c < NJ; ++c)
       if (4 * ty + r < w.L)
-        out[((w.tok0 + 4 * ty + r) * HV + hv) * V + tx + 16 * c] = from_f<T>(a.scale * o[r][c]);
+        out[((w.tok0 + 4 * ty + r) * HV + hv) * V + tx + 16 * c] = a.scale * o[r][c];
 }
 
 // sum over the 16 threads tx of a row group; every one of them gets it
@@ -255,18 +304,18 @@ GDN2_DEV float row_sum(float x) {
 
 // One CTA per (chunk, key head): the value heads of the group one after the
 // other, their shares of dq and dk added up in registers.
-template <typename T, int K, int V>
+template <int K, int V>
 __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args a, gdn2_linear_attn_grads gr,
                                                           LaDecay dec, LaGeom geo, const float* states,
                                                           const float* dstates, float* dgf) {
-  extern __shared__ float sm[];
+  extern __shared__ __align__(16) float sm[];
   float* Q = sm;
-  float* Kt = Q + kC * (K + 1);
-  float* Vt = Kt + kC * (K + 1);
-  float* D = Vt + kC * (V + 1);
-  float* P = D + kC * (V + 1);
+  float* Kt = Q + kC * (K + kPad);
+  float* Vt = Kt + kC * (K + kPad);
+  float* D = Vt + kC * (V + kPad);
+  float* P = D + kC * (V + kPad);
   float* E = P + kC * kLdP;
-  float* S = E + kC * kLdP;  // half of a state, [64][128 + 1] or [128][64 + 1]
+  float* S = E + kC * kLdP;  // half of a state, 64 rows, or 64 columns
   __shared__ double G[kC];
   __shared__ float colw[8][kC], rows[kC], qint[kC], kint[kC], wsum[8];
   Where w;
@@ -279,16 +328,16 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
   float dq[4][NK], dk[4][NK];
   zero(dq);
   zero(dk);
-  load_rows<T, K>(Q, static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.t0 * a.q_stride[1] + h * a.q_stride[2],
+  load_rows<K>(Q, static_cast<const float*>(a.q) + w.b * a.q_stride[0] + w.t0 * a.q_stride[1] + h * a.q_stride[2],
                   a.q_stride[1], w.L);
-  load_rows<T, K>(Kt, static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.t0 * a.k_stride[1] + h * a.k_stride[2],
+  load_rows<K>(Kt, static_cast<const float*>(a.k) + w.b * a.k_stride[0] + w.t0 * a.k_stride[1] + h * a.k_stride[2],
                   a.k_stride[1], w.L);
   for (int j = 0; j < group; ++j) {
     const int64_t hv = h * group + j;
     __syncthreads();
-    load_rows<T, V>(Vt, static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.t0 * a.v_stride[1] + hv * a.v_stride[2],
+    load_rows<V>(Vt, static_cast<const float*>(a.v) + w.b * a.v_stride[0] + w.t0 * a.v_stride[1] + hv * a.v_stride[2],
                     a.v_stride[1], w.L);
-    load_rows<T, V>(D, static_cast<const T*>(gr.dout) + (w.tok0 * HV + hv) * V, HV * V, w.L);
+    load_rows<V>(D, static_cast<const float*>(gr.dout) + (w.tok0 * HV + hv) * V, HV * V, w.L);
     chunk_sums(G, dec, w.b, w.t0, hv, w.L);
     __syncthreads();
     const float* st = states + ((int64_t)blockIdx.x * HV + hv) * K * V;
@@ -298,8 +347,8 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
       float p[4][4], e[4][4], col[4] = {0.f, 0.f, 0.f, 0.f};
       zero(p);
       zero(e);
-      tile_mm(p, Q, K + 1, 1, Kt, 1, K + 1, K);
-      tile_mm(e, D, V + 1, 1, Vt, 1, V + 1, V);
+      tile_mm<false, true>(p, Q, K + kPad, Kt, K + kPad, K);
+      tile_mm<false, true>(e, D, V + kPad, Vt, V + kPad, V);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float row = 0.f;
@@ -333,9 +382,9 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
       zero(acc);
       for (int k0 = 0; k0 < K; k0 += 64) {
         __syncthreads();
-        for (int i = threadIdx.x; i < 64 * V; i += kThreads) S[(i / V) * (V + 1) + i % V] = dst[k0 * V + i];
+        load_state<64, V>(S, dst + k0 * V, V);
         __syncthreads();
-        tile_mm(acc, Kt + k0, K + 1, 1, S, V + 1, 1, 64);
+        tile_mm<false, false>(acc, Kt + k0, K + kPad, S, V + kPad, 64);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -343,22 +392,22 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
 #pragma unroll
         for (int c = 0; c < NV; ++c) acc[r][c] *= f;
       }
-      tile_mm(acc, P, 1, kLdP, D, V + 1, 1, kC);
-      T* out = static_cast<T*>(gr.dv);
+      tile_mm<true, false>(acc, P, kLdP, D, V + kPad, kC);
+      float* out = static_cast<float*>(gr.dv);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < NV; ++c)
-          if (4 * ty + r < w.L) out[((w.tok0 + 4 * ty + r) * HV + hv) * V + tx + 16 * c] = from_f<T>(acc[r][c]);
+          if (4 * ty + r < w.L) out[((w.tok0 + 4 * ty + r) * HV + hv) * V + tx + 16 * c] = acc[r][c];
     }
     {  // dq += scale e^G do S^T + E k
       float acc[4][NK];
       zero(acc);
       for (int v0 = 0; v0 < V; v0 += 64) {
         __syncthreads();
-        for (int i = threadIdx.x; i < K * 64; i += kThreads) S[(i / 64) * 65 + i % 64] = st[(i / 64) * V + v0 + i % 64];
+        load_state<K, 64>(S, st + v0, V);
         __syncthreads();
-        tile_mm(acc, D + v0, V + 1, 1, S, 1, 65, 64);
+        tile_mm<false, true>(acc, D + v0, V + kPad, S, 64 + kPad, 64);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -367,14 +416,14 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
 #pragma unroll
         for (int c = 0; c < NK; ++c) {
           acc[r][c] *= f;
-          x = fmaf(acc[r][c], Q[(4 * ty + r) * (K + 1) + tx + 16 * c], x);
+          x = fmaf(acc[r][c], Q[(4 * ty + r) * (K + kPad) + tx + 16 * c], x);
         }
         if (want_dg) {
           x = row_sum(x);
           if (tx == 0) qint[4 * ty + r] = x;
         }
       }
-      tile_mm(acc, E, kLdP, 1, Kt, K + 1, 1, kC);
+      tile_mm<false, false>(acc, E, kLdP, Kt, K + kPad, kC);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -385,9 +434,9 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
       zero(acc);
       for (int v0 = 0; v0 < V; v0 += 64) {
         __syncthreads();
-        for (int i = threadIdx.x; i < K * 64; i += kThreads) S[(i / 64) * 65 + i % 64] = dst[(i / 64) * V + v0 + i % 64];
+        load_state<K, 64>(S, dst + v0, V);
         __syncthreads();
-        tile_mm(acc, Vt + v0, V + 1, 1, S, 1, 65, 64);
+        tile_mm<false, true>(acc, Vt + v0, V + kPad, S, 64 + kPad, 64);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -396,14 +445,14 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
 #pragma unroll
         for (int c = 0; c < NK; ++c) {
           acc[r][c] *= f;
-          x = fmaf(acc[r][c], Kt[(4 * ty + r) * (K + 1) + tx + 16 * c], x);
+          x = fmaf(acc[r][c], Kt[(4 * ty + r) * (K + kPad) + tx + 16 * c], x);
         }
         if (want_dg) {
           x = row_sum(x);
           if (tx == 0) kint[4 * ty + r] = x;
         }
       }
-      tile_mm(acc, E, 1, kLdP, Q, K + 1, 1, kC);
+      tile_mm<true, false>(acc, E, kLdP, Q, K + kPad, kC);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -411,43 +460,65 @@ __global__ void __launch_bounds__(kThreads) la_bwd_kernel(gdn2_linear_attn_args 
     }
     if (want_dg) {
       float x = 0.f;
-      for (int i = threadIdx.x; i < K * V; i += kThreads) x = fmaf(st[i], dst[i], x);
+#pragma unroll 4
+      for (int i = threadIdx.x; i < K * V / 4; i += kThreads) {
+        const float4 y = reinterpret_cast<const float4*>(st)[i], z = reinterpret_cast<const float4*>(dst)[i];
+        x = fmaf(y.x, z.x, x);
+        x = fmaf(y.y, z.y, x);
+        x = fmaf(y.z, z.z, x);
+        x = fmaf(y.w, z.w, x);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
       if (lane == 0) wsum[warp] = x;
       __syncthreads();
-      if (threadIdx.x < kC) {
-        float x0 = 0.f;
+      if (warp == 0) {  // two tokens per lane: sums to the chunk's end, and of kint from its start
+        float x0 = 0.f, e[2], k[2];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x0 += wsum[i];
-        const int t = threadIdx.x;
-        float d = expf((float)GC) * x0;
-        for (int i = t; i < kC; ++i) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int t = 2 * lane + u;
           float cs = 0.f;
 #pragma unroll
-          for (int ww = 0; ww < 8; ++ww) cs += colw[ww][i];
-          d += rows[i] + qint[i] - cs;
+          for (int ww = 0; ww < 8; ++ww) cs += colw[ww][t];
+          e[u] = rows[t] + qint[t] - cs;
+          k[u] = kint[t];
         }
-        for (int i = 0; i < t; ++i) d += kint[i];
-        if (t < w.L) {
-          const int64_t at = (w.tok0 + t) * HV + hv;
-          if (dgf) dgf[at] = d;
-          else if (a.dtype_g == GDN2_BF16) static_cast<__nv_bfloat16*>(gr.dg)[at] = __float2bfloat16_rn(d);
-          else static_cast<float*>(gr.dg)[at] = d;
+        float after = e[0] + e[1], before = k[0] + k[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float y = __shfl_down_sync(0xffffffffu, after, o), z = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane + o < 32) after += y;
+          if (lane >= o) before += z;
+        }
+        after = __shfl_down_sync(0xffffffffu, after, 1);
+        before = __shfl_up_sync(0xffffffffu, before, 1);
+        const float base = expf((float)GC) * x0 + (lane < 31 ? after : 0.f) + (lane ? before : 0.f) + e[1];
+        const float d[2] = {base + e[0], base + k[0]};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int t = 2 * lane + u;
+          if (t < w.L) {
+            const int64_t at = (w.tok0 + t) * HV + hv;
+            if (dgf) dgf[at] = d[u];
+            else if (a.dtype_g == GDN2_BF16) static_cast<__nv_bfloat16*>(gr.dg)[at] = __float2bfloat16_rn(d[u]);
+            else static_cast<float*>(gr.dg)[at] = d[u];
+          }
         }
       }
     }
   }
-  T* oq = static_cast<T*>(gr.dq);
-  T* ok = static_cast<T*>(gr.dk);
+  float* oq = static_cast<float*>(gr.dq);
+  float* ok = static_cast<float*>(gr.dk);
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int c = 0; c < NK; ++c)
       if (4 * ty + r < w.L) {
         const int64_t at = ((w.tok0 + 4 * ty + r) * H + h) * K + tx + 16 * c;
-        oq[at] = from_f<T>(dq[r][c]);
-        ok[at] = from_f<T>(dk[r][c]);
+        oq[at] = dq[r][c];
+        ok[at] = dk[r][c];
       }
 }
 
@@ -603,7 +674,7 @@ __global__ void __launch_bounds__(256) la_zero_outside_kernel(LaRows r, LaGeom g
   zero_outside(r, geo, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
-template <typename T, int K, int V>
+template <int K, int V>
 int fwd(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
   const LaGeom geo = la_geom(a, ws);
   const LaDecay dec = la_decay(a);
@@ -613,10 +684,10 @@ int fwd(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
   float* ht = (a.flags & GDN2_STORE_FINAL) ? a.ht : nullptr;
   ProfScope ps(kKLinAttnFp32, s);
   if (NT > 0) {
-    const size_t sm = kC * (K + 1 + V + 1) * 4;
-    if (int st = (smem_opt_in<la_state_kernel<T, K, V, false>>(sm))) return st;
-    la_state_kernel<T, K, V, false><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
-        static_cast<const T*>(a.k), a.k_stride[0], a.k_stride[1], a.k_stride[2], static_cast<const T*>(a.v),
+    const size_t sm = kC * (K + V + 2 * kPad) * 4;
+    if (int st = (smem_opt_in<la_state_kernel<K, V, false>>(sm))) return st;
+    la_state_kernel<K, V, false><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
+        static_cast<const float*>(a.k), a.k_stride[0], a.k_stride[1], a.k_stride[2], static_cast<const float*>(a.v),
         a.v_stride[0], a.v_stride[1], a.v_stride[2], dec, geo, HV, group, 1.f, ws.states, ws.total);
     GDN2_LAUNCH_CHECK();
   }
@@ -624,15 +695,15 @@ int fwd(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s) {
                                                                                           geo, HV, K * V);
   GDN2_LAUNCH_CHECK();
   if (NT > 0) {
-    const size_t sm = (2 * kC * (K + 1) + kC * (V + 1) + kC * kLdP + 64 * (V + 1)) * 4;
-    if (int st = (smem_opt_in<la_out_kernel<T, K, V>>(sm))) return st;
-    la_out_kernel<T, K, V><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(a, dec, geo, ws.states);
+    const size_t sm = (2 * kC * (K + kPad) + kC * (V + kPad) + kC * kLdP + 64 * (V + kPad)) * 4;
+    if (int st = (smem_opt_in<la_out_kernel<K, V>>(sm))) return st;
+    la_out_kernel<K, V><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(a, dec, geo, ws.states);
     GDN2_LAUNCH_CHECK();
   }
   return 0;
 }
 
-template <typename T, int K, int V>
+template <int K, int V>
 int bwd(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws, const LaBwdWs& bw,
         cudaStream_t s) {
   const LaGeom geo = la_geom(a, ws);
@@ -641,10 +712,10 @@ int bwd(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const 
   const int HV = (int)a.HV, group = (int)(a.HV / a.H);
   ProfScope ps(kKLinAttnFp32, s);
   if (NT > 0) {
-    const size_t sm = kC * (K + 1 + V + 1) * 4;
-    if (int st = (smem_opt_in<la_state_kernel<T, K, V, true>>(sm))) return st;
-    la_state_kernel<T, K, V, true><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
-        static_cast<const T*>(a.q), a.q_stride[0], a.q_stride[1], a.q_stride[2], static_cast<const T*>(gr.dout),
+    const size_t sm = kC * (K + V + 2 * kPad) * 4;
+    if (int st = (smem_opt_in<la_state_kernel<K, V, true>>(sm))) return st;
+    la_state_kernel<K, V, true><<<dim3((unsigned)NT, HV), kThreads, sm, s>>>(
+        static_cast<const float*>(a.q), a.q_stride[0], a.q_stride[1], a.q_stride[2], static_cast<const float*>(gr.dout),
         a.T * HV * V, (int64_t)HV * V, V, dec, geo, HV, group, a.scale, bw.dstates, nullptr);
     GDN2_LAUNCH_CHECK();
   }
@@ -652,28 +723,28 @@ int bwd(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const 
       bw.dstates, ws.total, gr.dht, gr.dh0, geo, HV, K * V);
   GDN2_LAUNCH_CHECK();
   if (NT > 0) {
-    constexpr int half = 64 * (V + 1) > K * 65 ? 64 * (V + 1) : K * 65;
-    const size_t sm = (2 * kC * (K + 1) + 2 * kC * (V + 1) + 2 * kC * kLdP + half) * 4;
-    if (int st = (smem_opt_in<la_bwd_kernel<T, K, V>>(sm))) return st;
-    la_bwd_kernel<T, K, V><<<dim3((unsigned)NT, (unsigned)a.H), kThreads, sm, s>>>(
+    constexpr int half = 64 * (V + kPad) > K * (64 + kPad) ? 64 * (V + kPad) : K * (64 + kPad);
+    const size_t sm = (2 * kC * (K + kPad) + 2 * kC * (V + kPad) + 2 * kC * kLdP + half) * 4;
+    if (int st = (smem_opt_in<la_bwd_kernel<K, V>>(sm))) return st;
+    la_bwd_kernel<K, V><<<dim3((unsigned)NT, (unsigned)a.H), kThreads, sm, s>>>(
         a, gr, dec, geo, ws.states, bw.dstates, a.decay == GDN2_DECAY_HEAD ? bw.dg : nullptr);
     GDN2_LAUNCH_CHECK();
   }
   return 0;
 }
 
-template <typename T, typename F>
+template <typename F>
 int by_dims(const gdn2_linear_attn_args& a, F f) {
-  if (a.K == 128) return a.V == 128 ? f.template operator()<T, 128, 128>() : f.template operator()<T, 128, 64>();
-  return a.V == 128 ? f.template operator()<T, 64, 128>() : f.template operator()<T, 64, 64>();
+  if (a.K == 128) return a.V == 128 ? f.template operator()<128, 128>() : f.template operator()<128, 64>();
+  return a.V == 128 ? f.template operator()<64, 128>() : f.template operator()<64, 64>();
 }
 
 struct FwdCall {
   const gdn2_linear_attn_args& a;
   const LaWs& ws;
   cudaStream_t s;
-  template <typename T, int K, int V>
-  int operator()() const { return fwd<T, K, V>(a, ws, s); }
+  template <int K, int V>
+  int operator()() const { return fwd<K, V>(a, ws, s); }
 };
 struct BwdCall {
   const gdn2_linear_attn_args& a;
@@ -681,8 +752,8 @@ struct BwdCall {
   const LaWs& ws;
   const LaBwdWs& bw;
   cudaStream_t s;
-  template <typename T, int K, int V>
-  int operator()() const { return bwd<T, K, V>(a, gr, ws, bw, s); }
+  template <int K, int V>
+  int operator()() const { return bwd<K, V>(a, gr, ws, bw, s); }
 };
 
 }  // namespace
@@ -710,7 +781,7 @@ int la_fwd_launch(const gdn2_linear_attn_args& a, const LaWs& ws, cudaStream_t s
     return 0;
   }
   if (la_tc(a)) return la_tc_fwd_launch(a, ws, s);
-  return by_dims<float>(a, FwdCall{a, ws, s});
+  return by_dims(a, FwdCall{a, ws, s});
 }
 
 int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& gr, const LaWs& ws,
@@ -733,7 +804,7 @@ int la_bwd_launch(const gdn2_linear_attn_args& a, const gdn2_linear_attn_grads& 
   }
   if (la_tc(a)) {
     if (int st = la_tc_bwd_launch(a, gr, ws, bw, s)) return st;
-  } else if (int st = by_dims<float>(a, BwdCall{a, gr, ws, bw, s})) {
+  } else if (int st = by_dims(a, BwdCall{a, gr, ws, bw, s})) {
     return st;
   }
   if (gr.dg && a.decay == GDN2_DECAY_HEAD) {
