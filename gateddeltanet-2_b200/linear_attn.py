@@ -43,7 +43,8 @@ def chunk_linear_attn(
     ``output_final_state``.  Differentiable in q, k, v, g and initial_state,
     through o and the final state.  With bf16 inputs o and the gradients of q,
     k, v, g carry bf16 operand rounding (fp32 accumulation); the final state
-    and the gradient of the initial state keep fp32 accuracy.  A non-finite
+    and the gradient of the initial state are within some 4e-6 of their size
+    (products of two bf16 terms per value).  A non-finite
     input may reach earlier outputs of its own chunk (at most 128 tokens), and
     nothing of other sequences.
     """
