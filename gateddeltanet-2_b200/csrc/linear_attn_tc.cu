@@ -186,10 +186,6 @@ GDN2_DEV void ld_32bytes(const float* p, float* x) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(r[e]);
 }
-// (16-byte aligned, a multiple of 16 bytes)
-GDN2_DEV void prefetch_l2(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
 // Bounded waits.  One lane: the retry loop is one copy of code.  A whole warp:
 // votes keep it converged in a way that the compiler can see (a call would not).
 __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity) { return tc::mbar_wait(bar, parity); }
@@ -346,7 +342,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
         if (!find_task<kBack>(p, id, t)) continue;
         const int b = p.geo.cu ? 0 : (int)t.n;
         if (t.head && p.init && t.z == 0)  // both slices' state, ahead of the task's turn
-          prefetch_l2(p.init + (t.n * p.a.HV + t.hv) * K * p.a.V, (uint32_t)(K * p.a.V * 4));
+          l2_prefetch(p.init + (t.n * p.a.HV + t.hv) * K * p.a.V, (int)(K * p.a.V * 4));
         for (int i = 0; i < t.ce - t.cb; ++i, ++it) {
           const uint32_t sx = it % NX, sy = it % NY;
           const int tt = tok(nth(i));
@@ -811,7 +807,8 @@ GDN2_DEV float dot16(const unsigned char* row_base, int p0, int row, const float
 // loads, and none of its products, runs beside this one's chain of products and row
 // passes; the nine products are 4600 of some 16000 clocks.  Sixteen row warps instead
 // of eight overlap the passes' TMEM latencies: 136 -> 127 us.  Measured at 4 sequences
-// of 4096 tokens, 16 heads, K = V = 128: 125 us (604 MB, 4.8 TB/s), 112 us without dg.
+// of 4096 tokens, 16 heads, K = V = 128: 125 us (604 MB, 4.8 TB/s), 112 us without dg
+// (the next chunk's tiles fetched into L2 beforehand: no change, so it is the chain).
 // ---------------------------------------------------------------------------
 enum Tile { kTQ = 0, kTK, kTO, kTV, kTS, kTD };  // q, k, do, v, S, dS'
 
