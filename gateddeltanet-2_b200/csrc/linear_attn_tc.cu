@@ -84,7 +84,7 @@ struct alignas(1024) ScanSmem {
   Sums f[2];
   float cw[kOut ? 320 : 4];  // column factors of the score warps, 32 (w + 1) for w = 0..3
   uint64_t full_x[NX], empty_x[NX], full_y[NY], empty_y[NY], f_full[2], f_empty[2], qk_full[2], p_full[2];
-  uint64_t yw_full[NB], ds_full[NB], ds_free, s_full, s_free, y_ready[NY], o_full[2], o_free, drained;
+  uint64_t yw_full[NB], ds_full[NB], ds_free, s_full, s_free, y_ready[NY], o_full[2], o_free[2], drained;
   uint32_t tbase;
 };
 
@@ -232,6 +232,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       tc::mbar_init(&sm.qk_full[i], 1);
       tc::mbar_init(&sm.p_full[i], 256);
       tc::mbar_init(&sm.o_full[i], 2);  // Q S and P V
+      tc::mbar_init(&sm.o_free[i], 128);
     }
     for (uint32_t i = 0; i < NB; ++i) {
       tc::mbar_init(&sm.yw_full[i], 128);
@@ -241,7 +242,6 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
     tc::mbar_init(&sm.s_full, 128);
     tc::mbar_init(&sm.s_free, 1);
     tc::mbar_init(&sm.drained, kOut ? 2 : 1);  // one per issuer
-    tc::mbar_init(&sm.o_free, 128);
     tc::mbar_fence_init();
   }
   if (warp == 1) tc::tmem_alloc(&sm.tbase, kCols);
@@ -400,7 +400,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
         }
         if (it > 0) {
           const uint32_t j = it - 1, sj = j & 1, sy = j % NY;
-          if (j > 0 && !(ok = wait(&sm.o_free, (j - 1) & 1))) break;  // P V of the chunk before has left TMEM
+          if (j > 0 && !(ok = wait(&sm.o_free[(j - 1) & 1], ((j - 1) >> 1) & 1))) break;  // P V of the chunk before has left TMEM
           if (!(ok = wait(&sm.y_ready[sy], (j / NY) & 1) && wait(&sm.p_full[sj], (j >> 1) & 1))) break;
           tc::tc_fence_after();
 #pragma unroll
@@ -434,7 +434,10 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
             tc::mma_bf16(tb + kColDS + 64 * b, nmaj(ax, kk), nmaj(aW + (2 * b + e) * (kTile >> 4), kk), iDS, e + kk > 0);
         tc::mma_commit(&sm.ds_full[b]);
         if constexpr (kOut) {
-          if (it >= 2 && !(ok = wait(&sm.o_free, it & 1))) break;  // Q S of two chunks before has left TMEM
+          // Q S of two chunks before has left TMEM.  (A barrier per buffer: its next phase needs the
+          // Q S below.  With one barrier for both, the output of the chunk between, which needs nothing
+          // more from this warp, could end its phase first, and this wait would see the other parity.)
+          if (it >= 2 && !(ok = wait(&sm.o_free[s], ((it >> 1) & 1) ^ 1))) break;
           if (!(ok = wait(&sm.s_full, it & 1))) break;
           tc::tc_fence_after();
 #pragma unroll
@@ -704,7 +707,7 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
         if (dst) st_32bytes(dst + 16 * h, pack8(x), pack8(x + 8));
       }
       tc::tc_fence_before();
-      tc::mbar_arrive(&sm.o_free);
+      tc::mbar_arrive(&sm.o_free[d & 1]);
       return true;
     };
     for (int64_t id = blockIdx.x; id < tasks && ok; id += step) {
