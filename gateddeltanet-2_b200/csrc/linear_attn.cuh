@@ -50,6 +50,12 @@ struct LaGeom {
     }
   }
   GDN2_DEV int64_t chunk0(int64_t n) const { return cu ? (int64_t)first[n] : n * nts; }
+  // chunks of sequence n (a packed batch needs `first`), as far as the buffers hold them: all of
+  // them, unless offsets decrease and sequences overlap
+  GDN2_DEV int64_t chunks(int64_t n, int64_t len) const {
+    const int64_t all = (len + C - 1) / C;
+    return cu ? min(all, (int64_t)(first[n + 1] - first[n])) : all;
+  }
   // chunk id -> (sequence, chunk in it); false past the last chunk
   GDN2_DEV bool chunk(int64_t id, int64_t& n, int64_t& c) const {
     if (cu) {
@@ -88,6 +94,11 @@ struct LaSegs {
     return true;
   }
   GDN2_DEV int64_t first_of(int64_t n) const { return map ? (int64_t)first[n] : n * per; }
+  // segments of sequence n, as far as the buffers hold them
+  GDN2_DEV int64_t count(int64_t n, int64_t chunks) const {
+    const int64_t all = chunks > 0 ? (chunks + len - 1) / len : 1;
+    return map ? min(all, (int64_t)(first[n + 1] - first[n])) : all;
+  }
 };
 
 struct LaSegWs {

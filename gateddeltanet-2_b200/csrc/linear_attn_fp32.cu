@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(128) la_prefix_kernel(float* states, const flo
   if (e >= KV) return;
   int64_t bos, len;
   geo.seq(n, bos, len);
-  const int64_t nch = (len + kC - 1) / kC, c0 = geo.chunk0(n);
+  const int64_t nch = geo.chunks(n, len), c0 = geo.chunk0(n);
   float4 s = init ? *reinterpret_cast<const float4*>(init + nh * KV + e) : make_float4(0.f, 0.f, 0.f, 0.f);
   for (int64_t i0 = 0; i0 < nch; i0 += kAhead) {
     float4 add[kAhead];

@@ -120,12 +120,13 @@ GDN2_DEV bool find_task(const ScanArgs& p, int64_t id, Task& t) {
   int64_t s;
   if (!p.seg.get(t.entry, p.geo, t.n, s)) return false;
   p.geo.seq(t.n, t.bos, t.len);
-  const int nch = (int)((t.len + kC - 1) / kC);
-  t.chunk0 = p.geo.cu && !p.geo.first ? 0 : p.geo.chunk0(t.n);  // (used where states are stored)
+  const bool stored = !p.geo.cu || p.geo.first;  // states are: their rows have an end
+  const int nch = (int)(stored ? p.geo.chunks(t.n, t.len) : (t.len + kC - 1) / kC);
+  t.chunk0 = stored ? p.geo.chunk0(t.n) : 0;
   t.cb = (int)s * p.seg.len;
   t.ce = min(t.cb + p.seg.len, nch);
   const bool first = s == 0, last = t.ce >= nch;
-  t.head = kBack ? last : first;
+  t.head = kBack ? last || t.entry + 1 >= p.seg.entries : first;  // (entries end early where offsets decrease)
   t.tail = kBack ? first : last;
   if (p.pre && t.tail) return false;  // nobody needs the state that leaves the last segment
   return true;
@@ -743,7 +744,7 @@ __global__ void __launch_bounds__(128) la_segment_kernel(LaSegs seg, LaGeom geo,
   const int64_t n = blockIdx.x / HV, hv = blockIdx.x % HV;
   int64_t bos, len;
   geo.seq(n, bos, len);
-  const int64_t nch = (len + kC - 1) / kC, ns = nch > 0 ? (nch + seg.len - 1) / seg.len : 1;
+  const int64_t ns = seg.count(n, (len + kC - 1) / kC);
   const int64_t e0 = seg.first_of(n);
   if (ns < 3) return;  // the first segment's term is a whole state already, the last one's is not used
   for (int64_t e = ((int64_t)blockIdx.y * 128 + threadIdx.x) * 4; e < KV; e += (int64_t)gridDim.y * 512) {

@@ -1,0 +1,60 @@
+"""Calls of linear attention and layer norm at the edges of what they take: rows
+and batches that no sequence covers, offsets out of order, tensors off the
+16-byte grid, index types, other ways of differentiating."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def rand(seed, *shape, dtype=F32):
+    gen = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=gen).to(dtype).cuda()
+
+
+# ---------------------------------------------------------------------------
+# offsets that decrease
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,repeats", [(8192, 5), (1000, 3), (130, 9)])
+def test_decreasing_offsets_stay_in_the_workspace(gdn2, dtype, T, repeats):
+    """Overlapping sequences have more chunks and segments than the buffers hold: what follows the buffers stays as it was."""
+    L, lib = gdn2._lib, gdn2._lib.load()
+    H, K, V = 1, 64, 64
+    cu = torch.tensor([0, T] * repeats + [0, T], device="cuda")
+    N = len(cu) - 1
+    q, k, v, do = (rand(i, 1, T, H, K, dtype=dtype) for i in range(4))
+    g, h0, dht = -0.1 * rand(5, 1, T, H).abs(), rand(6, N, H, K, V), rand(7, N, H, K, V)
+    guard = 4 << 20
+
+    def room(n):  # n bytes and a guard after them
+        t = torch.zeros(n + guard, dtype=torch.uint8, device="cuda")
+        t[n:] = 0xA5
+        return t
+
+    def out(shape, dt):
+        n = torch.Size(shape).numel() * dt.itemsize
+        return room(n), n
+
+    o, ht, dq, dk, dv = out(q.shape, dtype), out(h0.shape, F32), out(q.shape, dtype), out(q.shape, dtype), out(q.shape, dtype)
+    dg, dh0 = out(g.shape, F32), out(h0.shape, F32)
+    st = dict(q_b=T * K, q_t=K, q_h=K, k_b=T * K, k_t=K, k_h=K, v_b=T * V, v_t=V, v_h=V, g_b=T, g_t=1, g_h=1)
+    a = L.LinearAttnArgs(B=1, T=T, H=H, HV=H, K=K, V=V, N=N, cu_seqlens=L.ptr(cu), scale=0.125,
+                         flags=L.HAS_H0 | L.STORE_FINAL | L.SAVE_FOR_BWD, dtype=L.BF16 if dtype == BF16 else L.F32,
+                         dtype_g=L.F32, decay=L.DECAY_TOKEN, q=L.ptr(q), k=L.ptr(k), v=L.ptr(v), g=L.ptr(g), h0=L.ptr(h0),
+                         ht=L.ptr(ht[0]), o=L.ptr(o[0]), **st)
+    gr = L.LinearAttnGrads(dout=L.ptr(do), dht=L.ptr(dht), dq=L.ptr(dq[0]), dk=L.ptr(dk[0]), dv=L.ptr(dv[0]),
+                           dg=L.ptr(dg[0]), dh0=L.ptr(dh0[0]))
+    n = lib.gdn2_linear_attn_workspace_size(a)
+    nb = lib.gdn2_linear_attn_bwd_workspace_size(a)
+    ws, bws = (room(n), n), (room(nb), nb)
+    stream = L.stream_ptr(q.device)
+    assert lib.gdn2_linear_attn_fwd(a, L.ptr(ws[0]), n, stream) == 0
+    assert lib.gdn2_linear_attn_bwd(a, gr, L.ptr(ws[0]), n, L.ptr(bws[0]), nb, stream) == 0
+    torch.cuda.synchronize()
+    assert L.device_fault_read() == 0
+    for t, size in (o, ht, dq, dk, dv, dg, dh0, ws, bws):
+        assert (t[size:] == 0xA5).all()
