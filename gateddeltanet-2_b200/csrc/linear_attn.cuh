@@ -232,6 +232,29 @@ inline LaGeom la_geom(const gdn2_linear_attn_args& a, const LaWs& ws) {
   return LaGeom{a.cu_seqlens, a.T, a.N, C, (a.T + C - 1) / C, ws.map, ws.first};
 }
 
+// Rows of packed tensors that lie in no sequence (before the first offset,
+// after the last) get zeros, a row by a CTA.  Offsets that cover the row, the usual case, leave nothing to do.
+struct LaRows {
+  void* p[4];
+  int64_t bytes[4];  // of one row
+};
+GDN2_DEV void zero_outside(const LaRows& r, const LaGeom& geo, int block, int blocks) {
+  int64_t b0, l0, b1, l1;
+  geo.seq(0, b0, l0);
+  geo.seq(geo.N - 1, b1, l1);
+  const int64_t end = b1 + l1, rows = b0 + (geo.T - end);
+  for (int64_t k = block; k < rows; k += blocks) {
+    const int64_t row = k < b0 ? k : end + (k - b0);
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      if (!r.p[i]) continue;
+      uint16_t* p = static_cast<uint16_t*>(r.p[i]) + row * (r.bytes[i] / 2);  // every row is a whole number of 2-byte units
+#pragma unroll 1
+      for (int64_t x = threadIdx.x; x < r.bytes[i] / 2; x += blockDim.x) p[x] = 0;
+    }
+  }
+}
+
 // The log-decay of one token.  Values below -150 (and -inf) count as -150: exp
 // of it is zero in fp32, and differences of running sums never become
 // inf - inf.  NaN stays NaN.

@@ -629,28 +629,6 @@ GDN2_DEV void order_entries(const LaGeom& geo, const LaSegs& seg, int32_t* order
   for (int64_t e = tid; e < seg.entries; e += 1024) order[atomicAdd(&count[cls(e)], 1)] = (int32_t)e;
 }
 
-// Rows of packed tensors that lie in no sequence (before the first offset,
-// after the last) get zeros.  Offsets that cover the row, the usual case, leave nothing to do.
-struct LaRows {
-  void* p[4];
-  int64_t bytes[4];  // of one row
-};
-GDN2_DEV void zero_outside(const LaRows& r, const LaGeom& geo, int64_t thread, int64_t threads) {
-  int64_t b0, l0, b1, l1;
-  geo.seq(0, b0, l0);
-  geo.seq(geo.N - 1, b1, l1);
-  const int64_t end = b1 + l1, rows = b0 + (geo.T - end);
-  if (rows <= 0) return;
-  for (int i = 0; i < 4; ++i) {
-    if (!r.p[i]) continue;
-    const int64_t units = r.bytes[i] / 2;  // every row is a whole number of 2-byte units
-    for (int64_t x = thread; x < rows * units; x += threads) {
-      const int64_t k = x / units, row = k < b0 ? k : end + (k - b0);
-      static_cast<uint16_t*>(r.p[i])[row * units + x % units] = 0;
-    }
-  }
-}
-
 // What a packed batch needs before its forward pass: CTA 0 lays out chunks and
 // segments, the others clear rows.  (One launch: they are a few microseconds each.)
 struct LaPacked {
@@ -663,7 +641,7 @@ struct LaPacked {
 };
 __global__ void __launch_bounds__(1024) la_packed_kernel(LaPacked p) {
   if (blockIdx.x > 0) {
-    zero_outside(p.rows, p.geo, (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
+    zero_outside(p.rows, p.geo, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
   if (p.map) chunk_map(p.geo, p.geo.C, 0, p.map, p.first, p.NT);
@@ -671,7 +649,7 @@ __global__ void __launch_bounds__(1024) la_packed_kernel(LaPacked p) {
   if (p.order) order_entries(p.geo, p.seg, p.order);
 }
 __global__ void __launch_bounds__(256) la_zero_outside_kernel(LaRows r, LaGeom geo) {
-  zero_outside(r, geo, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+  zero_outside(r, geo, blockIdx.x, gridDim.x);
 }
 
 template <int K, int V>

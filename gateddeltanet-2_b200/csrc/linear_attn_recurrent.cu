@@ -17,10 +17,11 @@ namespace gdn2 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kClear = 32;  // CTAs that clear rows outside of packed sequences
 
 template <typename T, int K, int VT>
 __global__ void __launch_bounds__(kThreads)
-la_recurrent_kernel(const gdn2_linear_attn_args a, const LaDecay dec, const LaGeom geo) {
+la_recurrent_kernel(const gdn2_linear_attn_args a, const LaDecay dec, const LaGeom geo, unsigned tiles_in_all) {
   constexpr int kGroups = VT / 4;                 // float4 columns of the tile
   constexpr int kRowSets = kThreads / kGroups;    // threads that share a column
   constexpr int kRows = K / kRowSets;             // rows per thread
@@ -29,6 +30,10 @@ la_recurrent_kernel(const gdn2_linear_attn_args a, const LaDecay dec, const LaGe
   __shared__ float s_decay;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t V = a.V, HV = a.HV;
+  if (blockIdx.x >= tiles_in_all) {  // packed batches: the last CTAs clear the rows that no sequence covers
+    zero_outside(LaRows{{a.o}, {HV * V * (int64_t)sizeof(T)}}, geo, blockIdx.x - tiles_in_all, kClear);
+    return;
+  }
   const int tiles = (int)(V / VT);
   const int64_t nh = blockIdx.x / tiles, n = nh / HV, hv = nh % HV, h = hv / (HV / a.H);
   const int v0 = (int)(blockIdx.x % tiles) * VT;
@@ -109,7 +114,8 @@ template <typename T, int K, int VT>
 int launch(const gdn2_linear_attn_args& a, cudaStream_t s) {
   const LaGeom geo{a.cu_seqlens, a.T, a.N, 1, a.T, nullptr, nullptr};
   ProfScope ps(kKLinAttnRec, s);
-  la_recurrent_kernel<T, K, VT><<<(unsigned)(a.N * a.HV * (a.V / VT)), kThreads, 0, s>>>(a, la_decay(a), geo);
+  const unsigned tiles = (unsigned)(a.N * a.HV * (a.V / VT));
+  la_recurrent_kernel<T, K, VT><<<tiles + (a.cu_seqlens ? kClear : 0), kThreads, 0, s>>>(a, la_decay(a), geo, tiles);
   GDN2_LAUNCH_CHECK();
   return 0;
 }

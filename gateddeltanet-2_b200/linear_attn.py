@@ -65,7 +65,8 @@ def fused_recurrent_linear_attn(
 ):
     r"""Token-by-token linear attention (inference only, no gradients).
 
-    Arguments as ``chunk_linear_attn``.  ``inplace_final_state`` writes the
+    Arguments as ``chunk_linear_attn`` (rows outside of every sequence get zeros
+    here too).  ``inplace_final_state`` writes the
     states back into ``initial_state`` (contiguous within a state), which is
     then also what is returned.  ``ssm_state_indices`` (``[N]``, with
     ``inplace_final_state``): sequence ``n`` reads and writes slot

@@ -58,3 +58,36 @@ def test_decreasing_offsets_stay_in_the_workspace(gdn2, dtype, T, repeats):
     assert L.device_fault_read() == 0
     for t, size in (o, ht, dq, dk, dv, dg, dh0, ws, bws):
         assert (t[size:] == 0xA5).all()
+
+
+# ---------------------------------------------------------------------------
+# rows that no sequence covers
+# ---------------------------------------------------------------------------
+def dirty(*like):
+    """Leaves NaN in the memory that the next allocations of these sizes get."""
+    for t in like:
+        for _ in range(3):
+            torch.full_like(t, float("nan"))
+
+
+def small(dtype, B=1, T=60, H=2, HV=4, K=64, V=128):
+    return (rand(1, B, T, H, K, dtype=dtype), rand(2, B, T, H, K, dtype=dtype), rand(3, B, T, HV, V, dtype=dtype),
+            -0.2 * rand(4, B, T, HV).abs())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("offsets", [[7, 20, 20, 50], [0, 30], [60, 60], [10, 11]])
+def test_recurrent_rows_outside_of_every_sequence_get_zeros(gdn2, dtype, offsets):
+    q, k, v, g = small(dtype)
+    cu = torch.tensor(offsets, device="cuda")
+    want, _ = gdn2.chunk_linear_attn(q, k, v, g, cu_seqlens=cu)
+    first, last = offsets[0], offsets[-1]
+    pool = rand(5, len(offsets), 4, 64, 128)
+    slots = torch.arange(len(offsets) - 1, device="cuda")
+    for kw in (dict(), dict(initial_state=pool.clone(), inplace_final_state=True, ssm_state_indices=slots),
+               dict(initial_state=pool.clone(), inplace_final_state=True, ssm_state_indices=slots - 1)):
+        dirty(v)
+        o, _ = gdn2.fused_recurrent_linear_attn(q, k, v, g, cu_seqlens=cu, **kw)
+        assert torch.isfinite(o).all() and not o[:, :first].any() and not o[:, last:].any()
+        if not kw:
+            assert (o.float() - want.float()).abs().max() <= 2.0 ** -6 * max(float(want.abs().max()), 1.0)
