@@ -91,3 +91,28 @@ def test_recurrent_rows_outside_of_every_sequence_get_zeros(gdn2, dtype, offsets
         assert torch.isfinite(o).all() and not o[:, :first].any() and not o[:, last:].any()
         if not kw:
             assert (o.float() - want.float()).abs().max() <= 2.0 ** -6 * max(float(want.abs().max()), 1.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_empty_batches_with_states(gdn2, dtype):
+    """No batch, no tokens: states of no elements have no address, which is no error."""
+    q, k, v, g = (t[:0] for t in small(dtype))
+    h0 = torch.zeros(0, 4, 64, 128, device="cuda")
+    for f in (gdn2.chunk_linear_attn, gdn2.fused_recurrent_linear_attn):
+        o, ht = f(q, k, v, g, initial_state=h0, output_final_state=True)
+        assert o.shape == v.shape and ht.shape == h0.shape
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, g, h0)]
+    o, ht = gdn2.chunk_linear_attn(*leaves[:4], initial_state=leaves[4], output_final_state=True)
+    grads = torch.autograd.grad([o, ht], leaves, [torch.ones_like(o), torch.ones_like(ht)])
+    assert all(x.shape == t.shape for x, t in zip(grads, leaves))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_pool_without_slots(gdn2, dtype):
+    """Every sequence is padding: zeros."""
+    q, k, v, g = small(dtype, B=3, T=1)
+    pool = torch.zeros(0, 4, 64, 128, device="cuda")
+    dirty(v)
+    o, p = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=pool, inplace_final_state=True,
+                                            ssm_state_indices=torch.full((3,), -1, device="cuda"))
+    assert p is pool and not o.any()
