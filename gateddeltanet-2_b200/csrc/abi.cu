@@ -72,6 +72,13 @@ int check_linear_attn(const gdn2_linear_attn_args* a, bool need_ptrs, bool need_
   return GDN2_OK;
 }
 
+// a call without sequences still has rows, all of them outside: zeros
+int clear(void* p, int64_t elements, int dtype, cudaStream_t s) {
+  if (!p || elements == 0) return GDN2_OK;
+  GDN2_CUDA_TRY(cudaMemsetAsync(p, 0, (size_t)elements * (dtype == GDN2_BF16 ? 2 : 4), s));
+  return GDN2_OK;
+}
+
 int check_layer_norm(const gdn2_layer_norm_args* a) {
   if (!a) return GDN2_ERR_NULL_POINTER;
   if (a->rows < 0 || a->rows >= (int64_t(1) << 31) || a->D < 1) return GDN2_ERR_SHAPE;
@@ -231,10 +238,11 @@ int gdn2_linear_attn_fwd(const gdn2_linear_attn_args* a, void* workspace, size_t
   if (a->state_indices) return GDN2_ERR_FLAGS;
   const size_t need = la_ws_layout(*a, nullptr, nullptr);
   if (need > workspace_bytes || (need > 0 && !workspace) || misaligned(workspace)) return GDN2_ERR_WORKSPACE;
-  if (a->N == 0) return GDN2_OK;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->N == 0) return clear(a->o, a->B * a->T * a->HV * a->V, a->dtype, s);
   LaWs ws;
   la_ws_layout(*a, workspace, &ws);
-  return la_fwd_launch(*a, ws, reinterpret_cast<cudaStream_t>(stream));
+  return la_fwd_launch(*a, ws, s);
 }
 
 int gdn2_linear_attn_bwd(const gdn2_linear_attn_args* a, const gdn2_linear_attn_grads* gr, const void* workspace,
@@ -253,12 +261,19 @@ int gdn2_linear_attn_bwd(const gdn2_linear_attn_args* a, const gdn2_linear_attn_
   if (need > workspace_bytes || (need > 0 && !workspace) || misaligned(workspace)) return GDN2_ERR_WORKSPACE;
   if (need_b > bwd_workspace_bytes || (need_b > 0 && !bwd_workspace) || misaligned(bwd_workspace))
     return GDN2_ERR_WORKSPACE;
-  if (a->N == 0) return GDN2_OK;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->N == 0) {
+    const int64_t rows = a->B * a->T;
+    for (void* p : {gr->dq, gr->dk})
+      if ((st = clear(p, rows * a->H * a->K, a->dtype, s))) return st;
+    if ((st = clear(gr->dv, rows * a->HV * a->V, a->dtype, s))) return st;
+    return clear(gr->dg, (a->decay == GDN2_DECAY_HEAD ? 1 : rows) * a->HV, a->dtype_g, s);
+  }
   LaWs ws;
   la_ws_layout(*a, const_cast<void*>(workspace), &ws);
   LaBwdWs bw;
   la_bwd_ws_layout(*a, bwd_workspace, &bw);
-  return la_bwd_launch(*a, *gr, ws, bw, reinterpret_cast<cudaStream_t>(stream));
+  return la_bwd_launch(*a, *gr, ws, bw, s);
 }
 
 int gdn2_linear_attn_recurrent_fwd(const gdn2_linear_attn_args* a, gdn2_stream_t stream) {
@@ -268,8 +283,9 @@ int gdn2_linear_attn_recurrent_fwd(const gdn2_linear_attn_args* a, gdn2_stream_t
   if (a->state_indices && a->num_slots < 0) return GDN2_ERR_SHAPE;
   if (a->state_stride_in % 4 || a->state_stride_out % 4) return GDN2_ERR_ALIGNMENT;
   if (a->N * a->HV * (a->V / 32) >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
-  if (a->N == 0) return GDN2_OK;
-  return la_recurrent_launch(*a, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->N == 0) return clear(a->o, a->B * a->T * a->HV * a->V, a->dtype, s);
+  return la_recurrent_launch(*a, s);
 }
 
 int gdn2_layer_norm_fwd(const gdn2_layer_norm_args* a, gdn2_stream_t stream) {

@@ -346,7 +346,8 @@ int gdn2_norm_gate_bwd(const void* dy, const void* x, const void* gate, const fl
  * dimension is contiguous, base addresses and the other strides are multiples
  * of 16 bytes.  g: no decay, one value per head, or one per token and head
  * (natural log; -inf forgets the state entirely).  Packed sequences as in
- * gdn2_chunk_fwd; spans outside [0, T) are clipped.  Offsets must not decrease:
+ * gdn2_chunk_fwd; spans outside [0, T) are clipped, and rows in no sequence get
+ * zeros in o and in the gradients.  Offsets must not decrease:
  * where they do, sequences overlap and results are unspecified, but nothing
  * outside of the buffers is read or written.
  * A token whose mask or length leaves a sequence empty contributes nothing:

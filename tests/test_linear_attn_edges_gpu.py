@@ -116,3 +116,29 @@ def test_pool_without_slots(gdn2, dtype):
     o, p = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=pool, inplace_final_state=True,
                                             ssm_state_indices=torch.full((3,), -1, device="cuda"))
     assert p is pool and not o.any()
+
+
+# ---------------------------------------------------------------------------
+# no sequences
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("decay", ["token", "head"])
+def test_tokens_but_no_sequences(gdn2, dtype, decay):
+    """cu_seqlens of one offset: every row lies outside, o and all gradients are zeros."""
+    q, k, v, g = small(dtype)
+    g = g if decay == "token" else g[0, 0].clone()
+    cu = torch.tensor([0], device="cuda")
+    h0 = torch.zeros(0, 4, 64, 128, device="cuda")
+    leaves = [t.requires_grad_() for t in (q, k, v, g, h0)]
+    dirty(v)
+    o, ht = gdn2.chunk_linear_attn(*leaves[:4], initial_state=h0, output_final_state=True, cu_seqlens=cu)
+    assert ht.shape == h0.shape and not o.any()
+    dirty(q, k, v, g)
+    grads = torch.autograd.grad([o, ht], leaves, [torch.ones_like(o), torch.ones_like(ht)])
+    assert all(not x.any() and x.shape == t.shape for x, t in zip(grads, leaves))
+    with torch.no_grad():
+        dirty(v)
+        assert not gdn2.chunk_linear_attn(q, k, v, g, cu_seqlens=cu)[0].any()
+        dirty(v)
+        o, ht = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True, cu_seqlens=cu)
+        assert not o.any() and ht.shape == h0.shape
