@@ -4,7 +4,9 @@ The plain sibling of ``GatedDeltaNet2``: one projection to q, k, v, linear
 attention (``chunk_linear_attn`` for training and prompts,
 ``fused_recurrent_linear_attn`` for up to 64 tokens outside training), a layer
 norm of each head's output, a SiLU gate and the output projection.  Same
-forward signature, return value and cache protocol as ``GatedDeltaNet2``.
+forward signature, return value and cache protocol as ``GatedDeltaNet2``: a
+0-1 ``attention_mask`` [B, T] (0: padding) takes padding tokens out before the
+projections, and their outputs are zeros.
 """
 
 from __future__ import annotations
@@ -15,6 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .layer import _unpad
 from .layer_norm import LayerNorm
 from .linear_attn import chunk_linear_attn, fused_recurrent_linear_attn
 
@@ -64,8 +67,17 @@ class LinearAttention(nn.Module):
             if isinstance(m, nn.Linear):
                 nn.init.xavier_uniform_(m.weight, gain=2 ** -2.5)
 
-    def forward(self, hidden_states, past_key_values=None, use_cache=False, cu_seqlens=None, **kwargs):
+    def forward(self, hidden_states, attention_mask=None, past_key_values=None, use_cache=False,
+                output_attentions=False, cu_seqlens=None, **kwargs):
         B, T, _ = hidden_states.shape
+        if attention_mask is not None:
+            if attention_mask.ndim != 2 or attention_mask.shape[0] != B or attention_mask.shape[1] < T:
+                raise ValueError(f"attention_mask must be a 0-1 matrix [batch, tokens] for padding, got "
+                                 f"{tuple(attention_mask.shape)} for hidden states {tuple(hidden_states.shape)}")
+            if cu_seqlens is not None:
+                raise ValueError("attention_mask and cu_seqlens cannot be given together")
+            indices, cu_seqlens = _unpad(attention_mask[:, -T:] if T else attention_mask[:, :0])
+            hidden_states = hidden_states.flatten(0, 1).index_select(0, indices).unsqueeze(0)
         state = None
         if past_key_values is not None:
             if self.layer_idx is None:
@@ -91,4 +103,7 @@ class LinearAttention(nn.Module):
             past_key_values.update(layer_idx=self.layer_idx, recurrent_state=state, offset=T)
         gate = self.g_proj(hidden_states).unflatten(-1, (self.num_v_heads, -1))
         o = self.o_norm(o) * F.silu(gate)
-        return self.o_proj(o.flatten(-2)), None, past_key_values
+        o = self.o_proj(o.flatten(-2))
+        if attention_mask is not None:
+            o = o.new_zeros(B * T, o.shape[-1]).index_copy(0, indices, o.squeeze(0)).view(B, T, -1)
+        return o, None, past_key_values

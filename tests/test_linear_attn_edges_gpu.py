@@ -142,3 +142,48 @@ def test_tokens_but_no_sequences(gdn2, dtype, decay):
         dirty(v)
         o, ht = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True, cu_seqlens=cu)
         assert not o.any() and ht.shape == h0.shape
+
+
+# ---------------------------------------------------------------------------
+# the mixer's padding mask
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("side", ["left", "right"])
+@pytest.mark.parametrize("T", [40, 90])
+def test_mixer_mask(gdn2, T, side):
+    """A padded batch against its sequences run alone, then a decode step on its states.  fp32
+    throughout: sums of at most 256 terms in another order, five in a row, stay below 1e-5."""
+    torch.manual_seed(0)
+    layer = gdn2.LinearAttention(hidden_size=256, head_dim=64, num_heads=2, num_v_heads=4, layer_idx=0).cuda().eval()
+    x, nxt = rand(1, 3, T, 256), rand(2, 3, 1, 256)
+    lens = [T, T - 29, 1]
+    mask = torch.zeros(3, T, dtype=torch.int64, device="cuda")
+    for i, n in enumerate(lens):
+        mask[i, slice(T - n, T) if side == "left" else slice(0, n)] = 1
+
+    def close(a, b):
+        assert float((a - b).norm()) <= 1e-5 * float(b.norm())
+
+    with torch.no_grad():
+        cache = gdn2.LayerCache()
+        o, none, same = layer(x, mask, cache, True)  # the older mixer's order of arguments
+        assert none is None and same is cache and not o[mask == 0].any()
+        for m in (mask.bool(), mask.float()):
+            assert torch.equal(layer(x, attention_mask=m)[0], o)
+        step = layer(nxt, attention_mask=torch.cat([mask, mask.new_ones(3, 1)], 1), past_key_values=cache, use_cache=True)[0]
+        for i in range(3):
+            alone = gdn2.LayerCache()
+            close(o[i][mask[i] == 1], layer(x[i:i + 1, mask[i] == 1], past_key_values=alone, use_cache=True)[0][0])
+            close(step[i], layer(nxt[i:i + 1], past_key_values=alone, use_cache=True)[0][0])
+            close(cache[0]["recurrent_state"][i], alone[0]["recurrent_state"][0])
+    # training: nothing flows to padding
+    leaf = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(layer.train()(leaf, attention_mask=mask)[0].square().sum(), leaf)
+    assert not dx[mask == 0].any()
+    for i in range(3):
+        one = x[i:i + 1, mask[i] == 1].clone().requires_grad_()
+        close(dx[i][mask[i] == 1], torch.autograd.grad(layer(one)[0].square().sum(), one)[0][0])
+    for bad in (mask[0], mask[:2], mask[:, :-1], mask[:, None]):
+        with pytest.raises(ValueError):
+            layer(x, attention_mask=bad)
+    with pytest.raises(ValueError):
+        layer(x[:1], attention_mask=mask[:1], cu_seqlens=torch.tensor([0, T], device="cuda"))
