@@ -48,6 +48,13 @@ void require_device(const Tensor& t) {
   seen.fetch_or(bit, std::memory_order_relaxed);
 }
 
+// Tangents would vanish without a trace: the kernels run on the values.
+void refuse_tangents(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                "linear attention and layer norm have no forward-mode derivative");
+}
+
 gdn2_stream_t stream_of(const Tensor& t) {
   return reinterpret_cast<gdn2_stream_t>(c10::cuda::getCurrentCUDAStream(t.get_device()).stream());
 }
@@ -127,6 +134,7 @@ int64_t check_attn(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
       {"k", &k}, {"v", &v}, {"g", &g}, {"initial_state", &h0}, {"cu_seqlens", &cu}};
   for (const auto& [name, t] : all)
     TORCH_CHECK_VALUE(!t->defined() || t->device() == q.device(), name, " is on ", t->device(), ", q on ", q.device(), ".");
+  refuse_tangents({&q, &k, &v, &g, &h0});
   require_device(q);
   return N;
 }
@@ -362,6 +370,7 @@ std::tuple<Tensor, OptTensor> layer_norm(const Tensor& x, const OptTensor& w0, c
                      x.scalar_type(), " or fp32, got ", r.scalar_type(), ".");
     TORCH_CHECK_VALUE(r.device() == x.device(), "residual is on ", r.device(), ", x on ", x.device(), ".");
   }
+  refuse_tangents({&x, &w, &b, &r});
   require_device(x);
   if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b) || wants(r))) {
     const variable_list out = LayerNorm::apply(x, w0, b0, eps, r0);

@@ -187,3 +187,25 @@ def test_mixer_mask(gdn2, T, side):
             layer(x, attention_mask=bad)
     with pytest.raises(ValueError):
         layer(x[:1], attention_mask=mask[:1], cu_seqlens=torch.tensor([0, T], device="cuda"))
+
+
+# ---------------------------------------------------------------------------
+# other ways of differentiating
+# ---------------------------------------------------------------------------
+def test_forward_mode_is_refused(gdn2):
+    """No tangent is computed: a dual input is an error, as for chunk_gdn2, and not a result without one."""
+    import torch.autograd.forward_ad as fwd
+    q, k, v, g = small(BF16)
+    h0 = rand(9, 1, 4, 64, 128)
+    x, w, b, r = rand(10, 20, 64), rand(11, 64), rand(12, 64), rand(13, 20, 64)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for i in range(5):
+            a = [dual(t) if i == j else t for j, t in enumerate((q, k, v, g, h0))]
+            for f in (gdn2.chunk_linear_attn, gdn2.fused_recurrent_linear_attn):
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    f(*a[:4], initial_state=a[4])
+        for i in range(4):
+            a = [dual(t) if i == j else t for j, t in enumerate((x, w, b, r))]
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                gdn2.layer_norm(a[0], a[1], a[2], residual=a[3])
