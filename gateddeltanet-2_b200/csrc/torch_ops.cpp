@@ -7,6 +7,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/grad_mode.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -53,6 +55,21 @@ void refuse_tangents(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
                                 "linear attention and layer norm have no forward-mode derivative");
+}
+
+// The gradients are not differentiable: under create_graph they lead to a node that
+// raises when it is reached on the way to an input or a cotangent, instead of counting as constants.
+variable_list once(const variable_list& cotangents, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  torch::autograd::edge_list edges = torch::autograd::get_current_node()->next_edges();
+  for (torch::autograd::Edge& e : torch::autograd::collect_next_edges(cotangents)) edges.push_back(std::move(e));
+  const auto error = std::make_shared<torch::autograd::Error>(
+      "the gradients of linear attention and layer norm cannot be differentiated", std::move(edges));
+  for (Tensor& t : grads) {
+    if (t.defined()) t = t.detach();
+    torch::autograd::set_history(t, error);
+  }
+  return grads;
 }
 
 gdn2_stream_t stream_of(const Tensor& t) {
@@ -214,7 +231,7 @@ struct ChunkLinearAttn : torch::autograd::Function<ChunkLinearAttn> {
     const Tensor bws = bytes(q, need);
     check(api.la_bwd(&a, &r, ptr(ws), ws.defined() ? (size_t)ws.numel() : 0, mptr(bws), need, stream_of(q)),
           "gdn2_linear_attn_bwd");
-    return {dq, dk, dv, dg, dh0, Tensor(), Tensor(), Tensor(), Tensor()};
+    return once(grads, {dq, dk, dv, dg, dh0, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -344,7 +361,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor ws = bytes(s, need);
     gdn2_layer_norm_grads g{dy.const_data_ptr(), ptr(ds), s.const_data_ptr(), mptr(dx), mptr(dr), mptr(dw), mptr(db)};
     check(api.ln_bwd(&a, &g, mptr(ws), need, stream_of(s)), "gdn2_layer_norm_bwd");
-    return {!need_x ? Tensor() : shared ? dr : dx, dw, db, Tensor(), dr};
+    return once(grads, {!need_x ? Tensor() : shared ? dr : dx, dw, db, Tensor(), dr});
   }
 };
 

@@ -27,7 +27,7 @@ def layer_norm(
     fp32 (one type), either may be None; residual: the shape of x, x's type or
     fp32.  Returns ``y`` in x's type, or ``(y, s)`` with a residual, ``s`` in
     the residual's type (s is rounded to it before the statistics).
-    Differentiable in every tensor (in reverse mode; forward-mode tangents are refused).
+    Differentiable in every tensor (once, in reverse mode; forward-mode tangents are refused).
     """
     y, s = _lib.ops().layer_norm(x, weight, bias, eps, residual)
     return y if residual is None else (y, s)

@@ -41,7 +41,7 @@ def chunk_linear_attn(
 
     Returns ``(o, final_state)``; ``final_state`` is None unless
     ``output_final_state``.  Differentiable in q, k, v, g and initial_state,
-    through o and the final state (in reverse mode; forward-mode tangents are
+    through o and the final state (once, in reverse mode; forward-mode tangents are
     refused).  With bf16 inputs o and the gradients of q,
     k, v, g carry bf16 operand rounding (fp32 accumulation); the final state
     and the gradient of the initial state are within some 4e-6 of their size

@@ -209,3 +209,16 @@ def test_forward_mode_is_refused(gdn2):
             a = [dual(t) if i == j else t for j, t in enumerate((x, w, b, r))]
             with pytest.raises((RuntimeError, NotImplementedError)):
                 gdn2.layer_norm(a[0], a[1], a[2], residual=a[3])
+
+
+def test_second_derivatives_are_refused(gdn2):
+    """The gradients are not differentiable: asking for their gradient is an error, not a missing term."""
+    q, k, v, g = (t.requires_grad_() for t in small(BF16))
+    o, _ = gdn2.chunk_linear_attn(q, k, v, g)
+    (dq,) = torch.autograd.grad(o.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.float().square().sum() + q.float().sum(), q)
+    x, w = rand(10, 20, 64).requires_grad_(), rand(11, 64).requires_grad_()
+    (dx,) = torch.autograd.grad(gdn2.layer_norm(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.square().sum() + x.sum(), x)
