@@ -287,6 +287,7 @@ std::tuple<Tensor, OptTensor> recurrent_linear_attn(const Tensor& q0, const Tens
   a.state_stride_in = h0.defined() ? h0.stride(0) : 0;
   a.state_stride_out = ht.defined() ? ht.stride(0) : 0;
   check(api.la_rec(&a, stream_of(o)), "gdn2_linear_attn_recurrent_fwd");
+  if (inplace && !h0.is_inference()) h0.unsafeGetTensorImpl()->bump_version();  // as every update in place
   return {o, inplace ? h00 : ht.defined() ? OptTensor(ht) : OptTensor()};
 }
 

@@ -222,3 +222,18 @@ def test_second_derivatives_are_refused(gdn2):
     (dx,) = torch.autograd.grad(gdn2.layer_norm(x, w).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dx.square().sum() + x.sum(), x)
+
+
+def test_a_state_updated_in_place_counts_as_changed(gdn2):
+    """A state that another function saved for its backward, then updated in place, is an error in that backward."""
+    q, k, v, g = small(BF16, T=1)
+    pool = rand(14, 1, 4, 64, 128)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    y = (w * pool).sum()  # saves the pool
+    before = pool._version
+    gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=pool, inplace_final_state=True)
+    assert pool._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=torch.zeros_like(pool), inplace_final_state=True)
