@@ -86,6 +86,10 @@ Tensor bytes(const Tensor& like, size_t n) {
 Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
 Tensor like(const Tensor& t, at::ScalarType dt) { return at::empty(t.sizes(), t.options().dtype(dt).requires_grad(false)); }
 bool off_grid(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) != 0; }
+// contiguous and on the 16-byte grid: `t` itself, or a copy (contiguous() alone returns a tensor off the grid as it is)
+Tensor on_grid(const Tensor& t) {
+  return !t.defined() || (t.is_contiguous() && !off_grid(t)) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 // ---------------------------------------------------------------------------
 // linear attention
@@ -190,7 +194,7 @@ Forward attn_forward(const Tensor& q0, const Tensor& k0, const Tensor& v0, const
   gdn2_linear_attn_args a{};
   Forward f;
   f.q = as_view(q0, a.q_stride), f.k = as_view(k0, a.k_stride), f.v = as_view(v0, a.v_stride);
-  f.h0 = h00.defined() ? h00.contiguous() : h00;
+  f.h0 = on_grid(h00);
   f.o = like(v0);
   if (final_state)
     f.ht = at::empty({N, v0.size(2), q0.size(3), v0.size(3)}, v0.options().dtype(at::kFloat).requires_grad(false));
@@ -220,8 +224,8 @@ struct ChunkLinearAttn : torch::autograd::Function<ChunkLinearAttn> {
     const Tensor qv = as_view(q, a.q_stride), kv = as_view(k, a.k_stride), vv = as_view(v, a.v_stride);
     fill(a, qv, kv, vv, g, h0, Tensor(), Tensor(), cu, ctx->saved_data["scale"].toDouble(), ctx->saved_data["n"].toInt(),
          GDN2_SAVE_FOR_BWD);
-    const Tensor dout = grads[0].defined() ? grads[0].contiguous() : at::zeros(v.sizes(), v.options());
-    const Tensor dht = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor dout = grads[0].defined() ? on_grid(grads[0]) : at::zeros(v.sizes(), v.options());
+    const Tensor dht = grads.size() > 1 ? on_grid(grads[1]) : Tensor();
     const Tensor dq = like(q), dk = like(k), dv = like(v);
     const int64_t need_grad = ctx->saved_data["need"].toInt();
     const Tensor dg = need_grad & 1 ? like(g) : Tensor(), dh0 = need_grad & 2 ? like(h0) : Tensor();
@@ -273,19 +277,21 @@ std::tuple<Tensor, OptTensor> recurrent_linear_attn(const Tensor& q0, const Tens
     a.state_indices = slots.const_data_ptr<int>();
   }
   const int64_t K = q0.size(3), V = v0.size(3);
+  const int64_t one = v0.size(2) * K * V;  // elements of a state
   if (h0.defined() && h0.numel() > 0 &&
-      (h0.stride(3) != 1 || h0.stride(2) != V || h0.stride(1) != K * V || h0.stride(0) % 4 || off_grid(h0))) {
+      (h0.stride(3) != 1 || h0.stride(2) != V || (h0.size(1) > 1 && h0.stride(1) != K * V) ||
+       (h0.size(0) > 1 && h0.stride(0) % 4) || off_grid(h0))) {
     TORCH_CHECK_VALUE(!inplace, "an initial_state that is updated in place must be contiguous within a state and 16-byte "
                                 "aligned");
-    h0 = h0.contiguous();
+    h0 = h0.clone(at::MemoryFormat::Contiguous);
   }
   const Tensor q = as_view(q0, a.q_stride), k = as_view(k0, a.k_stride), v = as_view(v0, a.v_stride), o = like(v0);
   if (inplace) ht = h0;
   else if (final_state) ht = at::empty({N, v0.size(2), K, V}, o.options().dtype(at::kFloat));
   const Tensor cu = as_offsets(get(cu0));
   fill(a, q, k, v, get(g), h0, ht, o, cu, scale.value_or(1.0 / std::sqrt((double)K)), N, 0);
-  a.state_stride_in = h0.defined() ? h0.stride(0) : 0;
-  a.state_stride_out = ht.defined() ? ht.stride(0) : 0;
+  a.state_stride_in = h0.defined() && h0.size(0) > 1 ? h0.stride(0) : one;  // (the step of a single state is never taken)
+  a.state_stride_out = ht.defined() && ht.size(0) > 1 ? ht.stride(0) : one;
   check(api.la_rec(&a, stream_of(o)), "gdn2_linear_attn_recurrent_fwd");
   if (inplace && !h0.is_inference()) h0.unsafeGetTensorImpl()->bump_version();  // as every update in place
   return {o, inplace ? h00 : ht.defined() ? OptTensor(ht) : OptTensor()};

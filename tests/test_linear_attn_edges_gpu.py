@@ -237,3 +237,58 @@ def test_a_state_updated_in_place_counts_as_changed(gdn2):
         y.backward()
     with torch.inference_mode():
         gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=torch.zeros_like(pool), inplace_final_state=True)
+
+
+# ---------------------------------------------------------------------------
+# tensors off the 16-byte grid
+# ---------------------------------------------------------------------------
+def off_grid(t):
+    """The same values in a contiguous tensor whose first element lies off the 16-byte grid."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    flat[1:] = t.flatten()
+    x = flat[1:].view(t.shape)
+    assert x.is_contiguous() and x.data_ptr() % 16
+    return x
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_states_and_cotangents_off_the_grid(gdn2, dtype):
+    q, k, v, g = small(dtype, B=2)
+    h0, do, dht = rand(6, 2, 4, 64, 128), rand(7, *v.shape, dtype=dtype), rand(8, 2, 4, 64, 128)
+
+    def once(f):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v, g)] + [f(h0).detach().requires_grad_()]
+        o, ht = gdn2.chunk_linear_attn(*leaves[:4], initial_state=leaves[4], output_final_state=True)
+        return [o, ht, *torch.autograd.grad([o, ht], leaves, [f(do), f(dht)])]
+
+    for a, b in zip(once(lambda t: t), once(off_grid)):
+        assert torch.equal(a, b)
+    a = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True)
+    b = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=off_grid(h0), output_final_state=True)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    with pytest.raises(ValueError):  # an update in place has to stay where it is
+        gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=off_grid(h0), inplace_final_state=True)
+
+
+def test_backward_through_a_cat_at_an_odd_place(gdn2):
+    q, k, v, g = small(BF16)
+    v.requires_grad_()
+    o, _ = gdn2.chunk_linear_attn(q, k, v, g)
+    weight = rand(9, o.numel(), dtype=BF16)
+    (want,) = torch.autograd.grad(o, v, weight.view(o.shape), retain_graph=True)
+    joined = torch.cat([torch.zeros(3, device="cuda", dtype=BF16), o.flatten()])
+    (dv,) = torch.autograd.grad(joined, v, torch.cat([weight[:3], weight]))
+    assert torch.equal(dv, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_sequence_with_an_odd_batch_step(gdn2, dtype):
+    """A dimension of one element may have any step: it is never taken."""
+    q, k, v, g = small(dtype)
+    n = 4 * 64 * 128
+    h0 = rand(6, n + 2).as_strided((1, 4, 64, 128), (n + 1, 64 * 128, 128, 1))
+    want = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0.clone(), output_final_state=True)
+    got = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    o, ht = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, inplace_final_state=True)
+    assert ht is h0 and torch.equal(o, want[0]) and torch.equal(h0, want[1])
