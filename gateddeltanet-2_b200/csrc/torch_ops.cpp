@@ -285,6 +285,8 @@ std::tuple<Tensor, OptTensor> recurrent_linear_attn(const Tensor& q0, const Tens
                                 "aligned");
     h0 = h0.clone(at::MemoryFormat::Contiguous);
   }
+  TORCH_CHECK_VALUE(!inplace || h0.size(0) < 2 || h0.stride(0) >= one, "states that are updated in place must not share "
+                                                                       "memory");
   const Tensor q = as_view(q0, a.q_stride), k = as_view(k0, a.k_stride), v = as_view(v0, a.v_stride), o = like(v0);
   if (inplace) ht = h0;
   else if (final_state) ht = at::empty({N, v0.size(2), K, V}, o.options().dtype(at::kFloat));

@@ -292,3 +292,16 @@ def test_one_sequence_with_an_odd_batch_step(gdn2, dtype):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     o, ht = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, inplace_final_state=True)
     assert ht is h0 and torch.equal(o, want[0]) and torch.equal(h0, want[1])
+
+
+def test_an_expanded_state_is_not_updated_in_place(gdn2):
+    """Sequences that share memory cannot each have a state there; reading it for all of them is fine."""
+    q, k, v, g = small(BF16, B=3, T=1)
+    h0 = rand(6, 1, 4, 64, 128).expand(3, 4, 64, 128)
+    want = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0.clone(), output_final_state=True)
+    got = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    half = rand(7, 4 * 4 * 64 * 128).as_strided((3, 4, 64, 128), (2 * 64 * 128, 64 * 128, 128, 1))  # half of each overlaps
+    for bad in (h0, half):
+        with pytest.raises(ValueError):
+            gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=bad, inplace_final_state=True)
