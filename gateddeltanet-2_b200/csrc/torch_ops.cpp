@@ -272,7 +272,7 @@ std::tuple<Tensor, OptTensor> recurrent_linear_attn(const Tensor& q0, const Tens
                           at::isIntegralType(slots.scalar_type(), false),
                       "ssm_state_indices must be a vector of ", N, " slots on ", q0.device());
     if (slots.scalar_type() != at::kInt || !slots.is_contiguous())
-      slots = slots.clamp(-1, INT32_MAX).to(at::kInt).contiguous();
+      slots = slots.to(at::kLong).clamp(-1, INT32_MAX).to(at::kInt).contiguous();
     a.num_slots = h0.size(0);
     a.state_indices = slots.const_data_ptr<int>();
   }

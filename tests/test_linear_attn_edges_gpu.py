@@ -305,3 +305,28 @@ def test_an_expanded_state_is_not_updated_in_place(gdn2):
     for bad in (h0, half):
         with pytest.raises(ValueError):
             gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=bad, inplace_final_state=True)
+
+
+# ---------------------------------------------------------------------------
+# types of slots
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("itype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_slot_types(gdn2, itype):
+    q, k, v, g = small(BF16, B=4, T=1)
+    pool = rand(5, 9, 4, 64, 128)
+    idx = torch.tensor([7, 100, 0, 3], device="cuda")
+    want = pool.clone()
+    ow, _ = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=want, inplace_final_state=True,
+                                             ssm_state_indices=idx.int())
+    o, _ = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=pool, inplace_final_state=True,
+                                            ssm_state_indices=idx.to(itype))
+    assert torch.equal(o, ow) and torch.equal(pool, want)
+
+
+def test_slots_beyond_32_bits_are_padding(gdn2):
+    q, k, v, g = small(BF16, B=3, T=1)
+    pool = rand(5, 4, 4, 64, 128)
+    keep = pool.clone()
+    idx = torch.tensor([2 ** 32, -2 ** 32 + 1, 2 ** 63 - 1], device="cuda")
+    o, _ = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=pool, inplace_final_state=True, ssm_state_indices=idx)
+    assert not o.any() and torch.equal(pool, keep)
