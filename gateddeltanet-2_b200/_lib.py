@@ -266,6 +266,17 @@ def ops():
     return _ops
 
 
+@torch.compiler.disable
+def _call_apart(name: str, *args):
+    return getattr(ops(), name)(*args)
+
+
+def call(name: str, *args):
+    """A torch function by its name; under a compiler the caller's graph breaks here, as at the ctypes
+    operators (asked only there: the decorator's wrapper costs an eager call 0.5 us)."""
+    return _call_apart(name, *args) if torch.compiler.is_compiling() else getattr(ops(), name)(*args)
+
+
 _checked_devices: set[int] = set()
 
 

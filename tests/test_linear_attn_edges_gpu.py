@@ -330,3 +330,24 @@ def test_slots_beyond_32_bits_are_padding(gdn2):
     idx = torch.tensor([2 ** 32, -2 ** 32 + 1, 2 ** 63 - 1], device="cuda")
     o, _ = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=pool, inplace_final_state=True, ssm_state_indices=idx)
     assert not o.any() and torch.equal(pool, keep)
+
+
+# ---------------------------------------------------------------------------
+# under a compiler
+# ---------------------------------------------------------------------------
+@pytest.mark.filterwarnings("error:Dynamo does not know how to trace")
+def test_traced_callers_run_the_operators_as_they_are(gdn2):
+    """A traced caller breaks its graph at these functions, as at the gated delta rule's."""
+    q, k, v, g = small(BF16)
+    q.requires_grad_()
+    w = rand(11, 128)
+
+    def f(q, k, v, g, w):
+        o, ht = gdn2.chunk_linear_attn(q * 1.0, k, v, g, output_final_state=True)
+        r, _ = gdn2.fused_recurrent_linear_attn(q.detach(), k, v, g)
+        return gdn2.layer_norm(o.float(), w) + r.float(), ht
+
+    want, want_ht = f(q, k, v, g, w)
+    got, ht = torch.compile(f, backend="eager")(q, k, v, g, w)
+    assert torch.equal(got, want) and torch.equal(ht, want_ht)
+    assert torch.equal(*(torch.autograd.grad(x.sum(), q)[0] for x in (got, want)))
