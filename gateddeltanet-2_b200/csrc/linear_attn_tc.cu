@@ -814,12 +814,15 @@ GDN2_DEV float dot16(const unsigned char* row_base, int p0, int row, const float
 // of 4096 tokens, 16 heads, K = V = 128: 125 us (604 MB, 4.8 TB/s), 112 us without dg
 // (the next chunk's tiles fetched into L2 beforehand: no change, so it is the chain).
 // ---------------------------------------------------------------------------
+constexpr float kLoUnit = 1.f / 16777216.f / 127.f;
+
 enum Tile { kTQ = 0, kTK, kTO, kTV, kTS, kTD };  // q, k, do, v, S, dS'
 
 struct alignas(1024) BwdSmem {
   __nv_bfloat16 slot[6][128 * 128];
   __nv_bfloat16 E[2][128 * 64];  // E^T, rows j
-  float hi[kC];                  // running sums of g
+  float hi[kC];                  // running sums of g, and
+  int8_t lo[kC];                 // what they miss, in 127ths of |hi| 2^-24 (half a unit in hi's last place at most)
   float g2[kC];                  // (G_i - G_{32 floor(i / 32)}) log2 e
   float r[kC];                   // 2^g2
   float xy[2][kC];               // X - Y, per half of the columns (two terms on a zero: their order is nothing)
@@ -1041,8 +1044,14 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
           g2[e] = (float)(G[e] - ref) * kLog2e;
           r[e] = exp2_approx(g2[e]);
         }
+        char4 lo;
+        auto rest = [&](int e) {  // (hi = 0: 0 times infinity is NaN, which converts to 0)
+          return (signed char)__float2int_rn((float)(G[e] - (double)hi[e]) * __frcp_rn(fabsf(hi[e]) * kLoUnit));
+        };
+        lo.x = rest(0), lo.y = rest(1), lo.z = rest(2), lo.w = rest(3);
         if (n > 0 && !(ok = warp_wait(&sm.f_empty, (n - 1) & 1))) break;
         reinterpret_cast<float4*>(sm.hi)[lane] = make_float4(hi[0], hi[1], hi[2], hi[3]);
+        reinterpret_cast<char4*>(sm.lo)[lane] = lo;
         reinterpret_cast<float4*>(sm.g2)[lane] = make_float4(g2[0], g2[1], g2[2], g2[3]);
         reinterpret_cast<float4*>(sm.r)[lane] = make_float4(r[0], r[1], r[2], r[3]);
         tc::mbar_arrive(&sm.f_full);
@@ -1127,9 +1136,12 @@ la_bwd_tc_kernel(const __grid_constant__ BwdArgs p, const __grid_constant__ CUte
         tc::mbar_arrive(&sm.clean);
         if (!(ok = warp_wait(&sm.f_full, par))) break;
         const float hj = sm.hi[row], gj = sm.g2[row], gc = sm.hi[kC - 1];
-        const float out_f = p.a.scale * exp_of(hj), in_f = exp_of(gc - hj);  // of the products with S and dS'
+        const float lj = sm.lo[row] * (fabsf(hj) * kLoUnit), hb = sm.hi[32 * quarter];
+        // of the products with S and dS'
+        const float out_f = p.a.scale * exp_of(hj), in_f = exp_of((gc - hj) + (sm.lo[kC - 1] * (fabsf(gc) * kLoUnit) - lj));
         const float eGC = exp_of(gc);
-        const float block_f = p.a.scale * exp_of(sm.hi[32 * quarter] - hj);  // of the 32 columns where quarter > q4
+        // of the 32 columns where quarter > q4
+        const float block_f = p.a.scale * exp_of((hb - hj) + (sm.lo[32 * quarter] * (fabsf(hb) * kLoUnit) - lj));
         float kdk = 0.f;  // k . dk, its part from within the chunk
         if (!(ok = warp_wait(&sm.g1, par))) break;
         tc::tc_fence_after();

@@ -351,3 +351,50 @@ def test_traced_callers_run_the_operators_as_they_are(gdn2):
     got, ht = torch.compile(f, backend="eager")(q, k, v, g, w)
     assert torch.equal(got, want) and torch.equal(ht, want_ht)
     assert torch.equal(*(torch.autograd.grad(x.sum(), q)[0] for x in (got, want)))
+
+
+# ---------------------------------------------------------------------------
+# strong decays
+# ---------------------------------------------------------------------------
+def test_decays_after_a_strong_burst_keep_their_bits(gdn2):
+    """64 tokens of decay -140 put the chunk's running sum near -9000, where floats are 2^-10 apart;
+    the factors between the tokens after them must not notice.
+
+    One nonzero term per value, operands of 1: an output is then its factor, rounded once to bf16 where
+    it goes through a product's operand (2^-8 of it at most) and not at all in the decays' gradient.  The factor
+    itself: 2^-22 from the exponential, differences of sums held to 2^-31 of 9000, an exponent of at
+    most 13 rounded a few times (2^-23 of it each): below 2e-5."""
+    T, H, K = 128, 32, 64
+    gen = torch.Generator().manual_seed(0)
+    g = torch.empty(1, T, H)
+    g[:, :64] = -140 + torch.rand(1, 64, H, generator=gen)
+    g[:, 64:] = -0.2 * torch.rand(1, 64, H, generator=gen)
+    G = g[0].double().cumsum(0)
+    one = torch.zeros(1, T, H, K)
+    one[..., 0] = 1.0
+    dev = lambda t: t.bfloat16().cuda().requires_grad_()  # noqa: E731
+
+    # the pairs (127, j): o of a value at j, and dv_j of a cotangent at 127
+    only = torch.zeros(1, T, H, K)
+    only[:, 127, :, 0] = 1.0
+    q, k, v, gl = dev(one), dev(one), dev(one), g.cuda().requires_grad_()
+    o, ht = gdn2.chunk_linear_attn(q, k, v, gl, scale=1.0, output_final_state=True)
+    dv, dk = torch.autograd.grad(o, (v, k), only.bfloat16().cuda(), retain_graph=True)
+    want = (G[127] - G[64:]).exp()
+    for name, x in (("dv", dv), ("dk", dk)):
+        err = (x[0, 64:, :, 0].detach().double().cpu() - want).abs() / want
+        assert float(err.max()) <= 2.0 ** -8 + 2e-5, (name, float(err.max()))
+
+    # the final state's cotangent and one key at 100: dg of every later token is that term's value
+    key = torch.zeros(1, T, H, K)
+    key[:, 100, :, 0] = 1.0
+    dht = torch.zeros(1, H, K, K)
+    dht[..., 0, 0] = 1.0
+    k = dev(key)
+    o, ht = gdn2.chunk_linear_attn(q, k, v, gl, scale=1.0, output_final_state=True)
+    (dg,) = torch.autograd.grad(ht, gl, dht.cuda())
+    want = (G[127] - G[100]).exp()
+    err = (dg[0, 101:].double().cpu() - want).abs() / want
+    assert float(err.max()) <= 2e-5, float(err.max())
+    err = (ht[0, :, 0, 0].detach().double().cpu() - want).abs() / want
+    assert float(err.max()) <= 2e-5, float(err.max())
