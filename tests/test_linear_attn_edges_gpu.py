@@ -398,3 +398,76 @@ def test_decays_after_a_strong_burst_keep_their_bits(gdn2):
     assert float(err.max()) <= 2e-5, float(err.max())
     err = (ht[0, :, 0, 0].detach().double().cpu() - want).abs() / want
     assert float(err.max()) <= 2e-5, float(err.max())
+
+
+# ---------------------------------------------------------------------------
+# the chunkwise form in a graph, and on two streams at once
+# ---------------------------------------------------------------------------
+def step(gdn2, q, k, v, g, h0, do, dht, cu=None):
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, g, h0)]
+    o, ht = gdn2.chunk_linear_attn(*leaves[:4], initial_state=leaves[4], output_final_state=True, cu_seqlens=cu)
+    return [o.detach(), ht.detach(), *torch.autograd.grad((o, ht), leaves, (do, dht))]
+
+
+def inputs(dtype, T, N, HV=4, seed=0, B=1):
+    H, K, V = 2, 64, 128
+    return [*(t.clone() for t in small(dtype, B=B, T=T, H=H, HV=HV)), rand(seed + 20, N, HV, K, V),
+            rand(seed + 21, B, T, HV, V, dtype=dtype), rand(seed + 22, N, HV, K, V)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,offsets", [(300, None), (5000, None), (400, [0, 130, 130, 131, 390])])
+def test_chunkwise_graph_capture(gdn2, dtype, T, offsets):
+    """A training step captured in a CUDA graph and replayed on new inputs, and new offsets."""
+    N = 1 if offsets is None else len(offsets) - 1
+    x = inputs(dtype, T, N)
+    cu = None if offsets is None else torch.tensor(offsets, device="cuda")
+    want = step(gdn2, *x, cu)
+    static = [torch.zeros_like(t) for t in x]
+    scu = None if cu is None else torch.linspace(0, T, N + 1, device="cuda").long()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(gdn2, *static, scu)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(gdn2, *static, scu)
+    for s, t in zip(static, x):
+        s.copy_(t)
+    if cu is not None:
+        scu.copy_(cu)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert gdn2._lib.device_fault_read() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_two_streams_at_once(gdn2, dtype):
+    """Calls in flight on two streams do not share scratch memory."""
+    data = [inputs(dtype, 700 + 300 * i, 1, seed=i) for i in range(2)]
+    want = [step(gdn2, *x) for x in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    got = [[] for _ in data]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(gdn2, *data[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    assert gdn2._lib.device_fault_read() == 0
+
+
+def test_long_fp32_prompt(gdn2):
+    """Many chunks of the fp32 form against the token-serial one: sums of some hundred terms in another order."""
+    T = 20000
+    q, k, v, g = small(F32, T=T, H=1, HV=1)
+    g = g * 0.02
+    h0 = rand(6, 1, 1, 64, 128)
+    o, ht = gdn2.chunk_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True)
+    o2, ht2 = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True)
+    for a, b in ((o, o2), (ht, ht2)):
+        assert float((a - b).norm()) <= 1e-5 * float(b.norm())
