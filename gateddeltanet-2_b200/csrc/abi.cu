@@ -58,7 +58,7 @@ int check_linear_attn(const gdn2_linear_attn_args* a, bool need_ptrs, bool need_
   if (a->cu_seqlens ? a->B != 1 : a->N != a->B) return GDN2_ERR_SHAPE;
   if (!need_ptrs) return GDN2_OK;
   if ((a->state_indices ? a->num_slots : a->N) > 0) {  // (tensors of no states have no address)
-    if ((a->flags & GDN2_HAS_H0) && !a->h0) return GDN2_ERR_NULL_POINTER;
+    if (need_out && (a->flags & GDN2_HAS_H0) && !a->h0) return GDN2_ERR_NULL_POINTER;
     if (need_out && (a->flags & GDN2_STORE_FINAL) && !a->ht) return GDN2_ERR_NULL_POINTER;
   }
   if (misaligned(a->h0) || misaligned(a->ht)) return GDN2_ERR_ALIGNMENT;

@@ -209,26 +209,29 @@ struct ChunkLinearAttn : torch::autograd::Function<ChunkLinearAttn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g,
                                const OptTensor& h0, const OptTensor& cu, double scale, bool final_state, int64_t N) {
     Forward f = attn_forward(q, k, v, get(g), get(h0), get(cu), scale, final_state, N, true);
-    ctx->save_for_backward({f.q, f.k, f.v, get(g), f.h0, get(cu), f.ws});
+    ctx->save_for_backward({f.q, f.k, f.v, get(g), get(cu), f.ws});  // (not h0: its values are not needed)
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["n"] = N;
-    ctx->saved_data["need"] = (int64_t)(wants(get(g)) | wants(get(h0)) << 1);
+    ctx->saved_data["need"] = (int64_t)(wants(get(g)) | wants(get(h0)) << 1 | h0.has_value() << 2);
     ctx->set_materialize_grads(false);
     return final_state ? variable_list{f.o, f.ht} : variable_list{f.o};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &g = s[3], &h0 = s[4], &cu = s[5], &ws = s[6];
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &g = s[3], &cu = s[4], &ws = s[5];
+    const int64_t N = ctx->saved_data["n"].toInt(), need_grad = ctx->saved_data["need"].toInt();
     const c10::cuda::CUDAGuard guard(q.device());
     gdn2_linear_attn_args a{};
     const Tensor qv = as_view(q, a.q_stride), kv = as_view(k, a.k_stride), vv = as_view(v, a.v_stride);
-    fill(a, qv, kv, vv, g, h0, Tensor(), Tensor(), cu, ctx->saved_data["scale"].toDouble(), ctx->saved_data["n"].toInt(),
-         GDN2_SAVE_FOR_BWD);
+    fill(a, qv, kv, vv, g, Tensor(), Tensor(), Tensor(), cu, ctx->saved_data["scale"].toDouble(), N,
+         GDN2_SAVE_FOR_BWD | (need_grad & 4 ? GDN2_HAS_H0 : 0));
     const Tensor dout = grads[0].defined() ? on_grid(grads[0]) : at::zeros(v.sizes(), v.options());
     const Tensor dht = grads.size() > 1 ? on_grid(grads[1]) : Tensor();
     const Tensor dq = like(q), dk = like(k), dv = like(v);
-    const int64_t need_grad = ctx->saved_data["need"].toInt();
-    const Tensor dg = need_grad & 1 ? like(g) : Tensor(), dh0 = need_grad & 2 ? like(h0) : Tensor();
+    const Tensor dg = need_grad & 1 ? like(g) : Tensor();
+    Tensor dh0;
+    if (need_grad & 2)
+      dh0 = at::empty({N, v.size(2), q.size(3), v.size(3)}, v.options().dtype(at::kFloat).requires_grad(false));
     gdn2_linear_attn_grads r{dout.const_data_ptr(), static_cast<const float*>(ptr(dht)), mptr(dq), mptr(dk), mptr(dv),
                              mptr(dg), static_cast<float*>(mptr(dh0))};
     const size_t need = api.la_bwd_ws(&a);

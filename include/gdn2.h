@@ -396,7 +396,9 @@ size_t gdn2_linear_attn_workspace_size(const gdn2_linear_attn_args* a);
 int gdn2_linear_attn_fwd(const gdn2_linear_attn_args* a, void* workspace, size_t workspace_bytes,
                          gdn2_stream_t stream);
 /* Backward; `workspace` as gdn2_linear_attn_fwd left it under GDN2_SAVE_FOR_BWD
- * for the same arguments.  Every gradient is reduced in a fixed order. */
+ * for the same arguments (h0, ht and o are not read and may be NULL; GDN2_HAS_H0
+ * says whether there was an initial state).  Every gradient is reduced in a fixed
+ * order. */
 size_t gdn2_linear_attn_bwd_workspace_size(const gdn2_linear_attn_args* a);
 int gdn2_linear_attn_bwd(const gdn2_linear_attn_args* a, const gdn2_linear_attn_grads* gr, const void* workspace,
                          size_t workspace_bytes, void* bwd_workspace, size_t bwd_workspace_bytes,

@@ -471,3 +471,34 @@ def test_long_fp32_prompt(gdn2):
     o2, ht2 = gdn2.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True)
     for a, b in ((o, o2), (ht, ht2)):
         assert float((a - b).norm()) <= 1e-5 * float(b.norm())
+
+
+def test_backward_after_the_initial_state_was_updated(gdn2):
+    """The backward does not read the initial state, so a decode step on it in between is no matter."""
+    q, k, v, g = small(BF16, T=100)
+    h0 = rand(6, 1, 4, 64, 128)
+    for dtype in (BF16, F32):
+        leaves = [t.to(dtype).requires_grad_() for t in (q, k, v)] + [g.clone().requires_grad_()]
+        S = h0.clone()
+        want = torch.autograd.grad(gdn2.chunk_linear_attn(*leaves, initial_state=S)[0].float().square().sum(), leaves)
+        o, _ = gdn2.chunk_linear_attn(*leaves, initial_state=S)
+        gdn2.fused_recurrent_linear_attn(*(t.detach()[:, :1] for t in leaves), initial_state=S, inplace_final_state=True)
+        S.zero_()
+        got = torch.autograd.grad(o.float().square().sum(), leaves)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_heads_before_tokens(gdn2, dtype):
+    """q, k, v laid out [B, H, T, D] in memory, and with the batch innermost of the three."""
+    x = [t.requires_grad_() for t in small(dtype, B=3, T=150)]
+    o, _ = gdn2.chunk_linear_attn(*x)
+    do = rand(9, *o.shape, dtype=dtype)
+    want = [o, *torch.autograd.grad(o, x, do), gdn2.fused_recurrent_linear_attn(*x)[0]]
+    for order in ((0, 2, 1, 3), (2, 1, 0, 3), (1, 0, 2, 3)):
+        back = [order.index(i) for i in range(4)]
+        y = [t.detach().permute(order).contiguous().permute(back).requires_grad_() for t in x[:3]] + [x[3]]
+        assert not y[0].is_contiguous()
+        o, _ = gdn2.chunk_linear_attn(*y)
+        got = [o, *torch.autograd.grad(o, y, do), gdn2.fused_recurrent_linear_attn(*y)[0]]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
