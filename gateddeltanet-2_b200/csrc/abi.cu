@@ -49,7 +49,8 @@ bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) !=
 int check_linear_attn(const gdn2_linear_attn_args* a, bool need_ptrs, bool need_out) {
   if (!a) return GDN2_ERR_NULL_POINTER;
   if (a->B < 0 || a->T < 0 || a->H <= 0 || a->HV <= 0 || a->N < 0 || a->HV % a->H) return GDN2_ERR_SHAPE;
-  if (a->HV > 65535 || a->B * a->T >= (int64_t(1) << 31) || a->N >= (int64_t(1) << 31)) return GDN2_ERR_SHAPE;
+  constexpr int64_t most = int64_t(1) << 31;
+  if (a->HV > 65535 || a->B * a->T >= most || a->N >= most || a->N * a->HV >= most) return GDN2_ERR_SHAPE;
   if (!dim_ok(a->K) || !dim_ok(a->V)) return GDN2_ERR_UNSUPPORTED_DIM;
   if (a->dtype != GDN2_BF16 && a->dtype != GDN2_F32) return GDN2_ERR_DTYPE;
   if (a->decay < GDN2_DECAY_NONE || a->decay > GDN2_DECAY_TOKEN) return GDN2_ERR_FLAGS;

@@ -95,3 +95,12 @@ def test_model_structure(gdn2):
     for n in ("transformer.ln_f.bias", "transformer.h.0.norm_1.bias", "transformer.h.0.attn.qkv_proj.weight",
               "transformer.h.0.attn.A_log", "transformer.h.0.attn.o_norm.weight", "transformer.h.1.attn.attn.weight"):
         assert n in names, n
+
+
+def test_more_states_than_a_grid_has_blocks(gdn2):
+    """N * HV blocks walk the states: 2^31 of them are refused, not taken modulo 2^32."""
+    lib = gdn2._lib.load()
+    a = _la(gdn2, B=1, T=100, N=1 << 29, cu_seqlens=16)
+    assert lib.gdn2_linear_attn_fwd(a, None, 0, None) == 2
+    assert lib.gdn2_linear_attn_recurrent_fwd(a, None) == 2
+    assert lib.gdn2_linear_attn_workspace_size(a) == 0
