@@ -11,6 +11,7 @@ import ctypes
 import os
 
 import torch
+from torch.compiler import is_dynamo_compiling
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgdn2_b200.so")
@@ -243,6 +244,23 @@ def stream_ptr(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx)
 
 
+class _Untraced:
+    """The same functions for a traced caller, whose graph breaks at them as at the ctypes operators."""
+
+    @torch.compiler.disable
+    def chunk_linear_attn(self, *args):
+        return ops().chunk_linear_attn(*args)
+
+    @torch.compiler.disable
+    def recurrent_linear_attn(self, *args):
+        return ops().recurrent_linear_attn(*args)
+
+    @torch.compiler.disable
+    def layer_norm(self, *args):
+        return ops().layer_norm(*args)
+
+
+_untraced = _Untraced()
 _ops = None
 OPS_PATH = os.path.join(_HERE, "_torch_ops.so")
 
@@ -250,6 +268,8 @@ OPS_PATH = os.path.join(_HERE, "_torch_ops.so")
 def ops():
     """The torch functions of csrc/torch_ops.cpp (linear attention, layer norm), bound to the loaded library."""
     global _ops
+    if is_dynamo_compiling():  # (asked here: a decorator's wrapper would cost every eager call 0.5 us)
+        return _untraced
     if _ops is None:
         if not os.path.exists(OPS_PATH):
             raise ImportError(f"{OPS_PATH} is missing: build it with `python gateddeltanet-2_b200/build.py`")
@@ -264,17 +284,6 @@ def ops():
             "status_string", "device_supported")])
         _ops = mod
     return _ops
-
-
-@torch.compiler.disable
-def _call_apart(name: str, *args):
-    return getattr(ops(), name)(*args)
-
-
-def call(name: str, *args):
-    """A torch function by its name; under a compiler the caller's graph breaks here, as at the ctypes
-    operators (asked only there: the decorator's wrapper costs an eager call 0.5 us)."""
-    return _call_apart(name, *args) if torch.compiler.is_compiling() else getattr(ops(), name)(*args)
 
 
 _checked_devices: set[int] = set()

@@ -29,7 +29,7 @@ def layer_norm(
     the residual's type (s is rounded to it before the statistics).
     Differentiable in every tensor (once, in reverse mode; forward-mode tangents are refused).
     """
-    y, s = _lib.call("layer_norm", x, weight, bias, eps, residual)
+    y, s = _lib.ops().layer_norm(x, weight, bias, eps, residual)
     return y if residual is None else (y, s)
 
 

@@ -49,7 +49,7 @@ def chunk_linear_attn(
     input may reach earlier outputs of its own chunk (at most 128 tokens), and
     nothing of other sequences.
     """
-    return _lib.call("chunk_linear_attn", q, k, v, g, scale, initial_state, output_final_state, cu_seqlens)
+    return _lib.ops().chunk_linear_attn(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens)
 
 
 def fused_recurrent_linear_attn(
@@ -75,5 +75,5 @@ def fused_recurrent_linear_attn(
     V]``; slots must differ, and a sequence whose slot is outside the pool
     (say -1, padding) is skipped and gets zero output.  Returns ``(o, final_state)``.
     """
-    return _lib.call("recurrent_linear_attn", q, k, v, g, scale, initial_state, output_final_state, inplace_final_state,
-                     cu_seqlens, ssm_state_indices)
+    return _lib.ops().recurrent_linear_attn(q, k, v, g, scale, initial_state, output_final_state, inplace_final_state,
+                                            cu_seqlens, ssm_state_indices)
