@@ -135,8 +135,8 @@ inline int64_t la_num_chunks(const gdn2_linear_attn_args& a) {
   return a.cu_seqlens ? a.T / C + a.N : a.B * ((a.T + C - 1) / C);
 }
 
-// The cut of the scans: enough segments for one per SM and 64-column slice of a
-// head, none shorter than 4 chunks.  A cut costs a second pass over k and v and two
+// The cut of the scans: as many segments as SMs for each 64-column slice of a
+// head (rounded down: 16 heads of 128 get 4, 128 tasks for 148 SMs), none shorter than 4 chunks.  A cut costs a second pass over k and v and two
 // launches, so it has to take two segments and 8 chunks off the walk.  One sequence,
 // 16 heads, K = V = 128, uncut and cut: 1024 tokens 22 and 30 us (2 x 4 chunks: not
 // cut), 2048 tokens 37 and 33 us (4 x 4; 2 x 8: 41 us), 16384 tokens 261 and 121 us;

@@ -10,6 +10,9 @@
 // at K = 128, four CTAs an SM.
 // Bound by bandwidth: 256 sequences of 16 heads, K = V = 128 (541 MB) take 88 us,
 // 6.15 TB/s; four sequences 8 us, which is the launch and one trip to memory and back.
+// Several tokens: each one's q, k, v are loaded after the barrier that ends the token
+// before, so a call of one sequence, 16 heads, takes 0.8 us a token (53 us for 64).
+// The last CTAs of a packed batch clear the rows outside of every sequence.
 #include "linear_attn.cuh"
 #include "profile.cuh"
 

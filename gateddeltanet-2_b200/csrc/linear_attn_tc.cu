@@ -29,6 +29,7 @@
 // Precision: P and S are rounded to bf16 as MMA operands (as the result itself
 // is).  w v goes in as the sum of two bf16 values, so the fp32 state carries 16
 // bits or more of every product: with one it would hold 8, and o as many again less.
+// (An infinite v makes the second value, a difference of infinities, NaN.)
 // Why 64 columns of V a CTA: two score buffers (256 TMEM columns), Q S of two
 // chunks (128), P V (64) and the state's term (64) then fill TMEM's 512 exactly, the
 // stages fill shared memory, and a sequence has twice as many CTAs; the price is
@@ -37,8 +38,10 @@
 // and read their operands from shared memory for some 2950 (K = 128); the roles'
 // hand-overs bring that to 3400 (batches in L2) to 4300.  Measured at 16 heads, K = V = 128:
 // 4 sequences of 4096 tokens 76 us (268 MB, 3.5 TB/s; 83 us where the states are kept
-// for the backward, 48 us for the reverse scan without outputs); 65536 tokens 277 us
-// after 138 us for the segments' own states; 23 packed sequences of 9001 tokens 74 us.
+// for the backward, 48 us for the reverse scan without outputs); 65536 tokens 267 us
+// after 139 us for the segments' own states (4 segments: 128 CTAs of 148 have a task, 96
+// in the first pass, where the last segments have none); 23 packed sequences of 9001
+// tokens 74 us.  Without outputs the same four warps make w v and then update the state.
 // Every wait is bounded (tc::kWaitLimitNs); one that gives up sets g_la_fault.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -807,7 +810,8 @@ GDN2_DEV float dot16(const unsigned char* row_base, int p0, int row, const float
 // chunk's q, k and do while this one is being finished, then k, q and do for its v, S and dS'.
 //   warp 0 loads, warp 1 dg, warp 2 running sums, warp 3 MMAs,
 //   warps 4-19: thread = token (TMEM lane) and a quarter of the columns
-// What bounds it: a chunk's six tiles fill shared memory, so little of the next one's
+// What bounds it: a chunk's six tiles fill shared memory at K = V = 128 (and have the same
+// room at 64, where two chunks' would fit), so little of the next one's
 // loads, and none of its products, runs beside this one's chain of products and row
 // passes; the nine products are 4600 of some 16000 clocks.  Sixteen row warps instead
 // of eight overlap the passes' TMEM latencies: 136 -> 127 us.  Measured at 4 sequences

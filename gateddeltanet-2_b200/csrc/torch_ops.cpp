@@ -1,9 +1,10 @@
 // The linear-attention and layer-norm operators as torch functions: argument
 // checks, allocation, autograd.  The work goes through the C ABI of gdn2.h,
 // whose functions `init` receives as addresses from the loaded library.
-// In C++ because a small call's cost is this layer: a decode step 24 -> 9 us, a
-// layer norm's forward and backward on few rows 125 -> 50 us against the same in Python
-// (autograd runs a C++ backward without the interpreter).
+// In C++ because a small call's cost is this layer: a decode step 24 -> 8 us, a
+// layer norm's forward and backward on few rows 125 -> 68 us against the same in Python
+// (autograd runs a C++ backward without the interpreter; torch's own product of two
+// tensors with its gradient takes 50 us on the same machine).
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>

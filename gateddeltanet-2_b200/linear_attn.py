@@ -42,12 +42,12 @@ def chunk_linear_attn(
     Returns ``(o, final_state)``; ``final_state`` is None unless
     ``output_final_state``.  Differentiable in q, k, v, g and initial_state,
     through o and the final state (once, in reverse mode; forward-mode tangents are
-    refused).  With bf16 inputs o and the gradients of q,
-    k, v, g carry bf16 operand rounding (fp32 accumulation); the final state
-    and the gradient of the initial state are within some 4e-6 of their size
-    (products of two bf16 terms per value).  A non-finite
-    input may reach earlier outputs of its own chunk (at most 128 tokens), and
-    nothing of other sequences.
+    refused).  With bf16 inputs o and the gradients of q, k, v, g carry bf16
+    operand rounding (fp32 accumulation); the final state and the gradient of
+    the initial state are within 1e-5 of their size, 4e-6 as a rule (products of
+    two bf16 terms per value).  A non-finite input may reach earlier outputs of
+    its own chunk (at most 128 tokens), and nothing of other sequences; an
+    infinity may come out as NaN.
     """
     return _lib.ops().chunk_linear_attn(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens)
 
