@@ -29,7 +29,6 @@
 // Precision: P and S are rounded to bf16 as MMA operands (as the result itself
 // is).  w v goes in as the sum of two bf16 values, so the fp32 state carries 16
 // bits or more of every product: with one it would hold 8, and o as many again less.
-// (An infinite v makes the second value, a difference of infinities, NaN.)
 // Why 64 columns of V a CTA: two score buffers (256 TMEM columns), Q S of two
 // chunks (128), P V (64) and the state's term (64) then fill TMEM's 512 exactly, the
 // stages fill shared memory, and a sequence has twice as many CTAs; the price is
@@ -296,10 +295,11 @@ la_scan_kernel(const __grid_constant__ ScanArgs p, const __grid_constant__ CUten
       const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t h = tc::bmul2(v[e], fh);
-        // what the product of the leading parts lost (exact), and the trailing part's product
-        wl[4 * q + e] = tc::bfma2(v[e], fl, tc::bfma2(v[e], fh, h ^ 0x80008000u));
-        wh[4 * q + e] = h;
+        wh[4 * q + e] = tc::bmul2(v[e], fh);
+        // what the product of the leading parts lost (exact), and the trailing part's product; of an
+        // infinity, which the leading part carries, those of the largest finite value: not inf - inf
+        const uint32_t u = tc::bmin_abs2(v[e], 0x7f7f7f7fu);
+        wl[4 * q + e] = tc::bfma2(u, fl, tc::bfma2(u, fh, tc::bmul2(u, fh) ^ 0x80008000u));
       }
     }
     return true;

@@ -341,6 +341,12 @@ __device__ __forceinline__ uint32_t bmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// each value's sign with the smaller of both magnitudes
+__device__ __forceinline__ uint32_t bmin_abs2(uint32_t a, uint32_t positive) {
+  uint32_t r;
+  asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(positive));
+  return r;
+}
 __device__ __forceinline__ uint32_t bfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));

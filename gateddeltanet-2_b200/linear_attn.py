@@ -47,7 +47,8 @@ def chunk_linear_attn(
     the initial state are within 1e-5 of their size, 4e-6 as a rule (products of
     two bf16 terms per value).  A non-finite input may reach earlier outputs of
     its own chunk (at most 128 tokens), and nothing of other sequences; an
-    infinity may come out as NaN.
+    infinite value stays one in the state unless a decay after it underflows
+    (zero times it is NaN).
     """
     return _lib.ops().chunk_linear_attn(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens)
 

@@ -502,3 +502,24 @@ def test_heads_before_tokens(gdn2, dtype):
         o, _ = gdn2.chunk_linear_attn(*y)
         got = [o, *torch.autograd.grad(o, y, do), gdn2.fused_recurrent_linear_attn(*y)[0]]
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------
+# infinities
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_an_infinite_value_is_infinite_in_the_state(gdn2, dtype):
+    """Infinite values in a column: k (+-inf) in that column of the final state, and nothing of it in the others."""
+    q, k, v, g = small(dtype, T=300)
+    k = torch.where(k == 0, torch.ones_like(k), k)
+    v = v.clone()
+    v[0, 290, 1, 5], v[0, 130, 2, 70] = float("inf"), -float("inf")
+    g = 0.01 * g  # far from underflow over the whole length
+    clean = v.clone()
+    clean[0, 290, 1, 5] = clean[0, 130, 2, 70] = 0.0
+    _, want = gdn2.chunk_linear_attn(q, k, clean, g, output_final_state=True)
+    _, ht = gdn2.chunk_linear_attn(q, k, v, g, output_final_state=True)
+    want = want.clone()
+    want[0, 1, :, 5] = float("inf") * k[0, 290, 0].sign().float()
+    want[0, 2, :, 70] = -float("inf") * k[0, 130, 1].sign().float()
+    assert torch.equal(ht, want)
